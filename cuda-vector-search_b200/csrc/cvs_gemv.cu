@@ -82,6 +82,10 @@ __global__ void __launch_bounds__(kGemvThreads) gemv_topk_kernel(const GemvArgs 
   const int chunks = a.d_pad >> 3;  // 16-byte chunks per row
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
 
+  // The queries were written by the kernel this one has just waited for: ordinary
+  // loads, which stay behind the wait. (Read-only-path loads may be moved ahead of
+  // it; at 8 queries of 384 columns the first query's were, and a search scheduled
+  // while its predecessor finished ran with that search's first query.)
   uint4 qv[NQ][CPL];
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi)
@@ -89,7 +93,7 @@ __global__ void __launch_bounds__(kGemvThreads) gemv_topk_kernel(const GemvArgs 
     for (int j = 0; j < CPL; ++j) {
       const int c = lane + 32 * j;
       qv[qi][j] = (qi < a.b && c < chunks)
-                      ? __ldg(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(qi) * a.d_pad) + c)
+                      ? *(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(qi) * a.d_pad) + c)
                       : zero;
     }
 
