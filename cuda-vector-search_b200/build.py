@@ -30,7 +30,9 @@ INCLUDE = REPO / "include"
 BUILD = HERE / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CU_SOURCES = ["cvs_tc_search.cu", "cvs_tc_pair.cu", "cvs_gemv.cu", "cvs_merge.cu", "cvs_ingest.cu", "cvs_capi.cu"]
+CU_SOURCES = ["cvs_tc_search.cu", "cvs_tc_pair.cu", "cvs_gemv.cu", "cvs_merge.cu", "cvs_ingest.cu", "cvs_capi.cu",
+              "cvs_norm.cu", "cvs_linear.cu", "cvs_preference.cu", "cvs_adapter_capi.cu"]
+EXT_SOURCES = ["torch_ext.cpp", "torch_adapter.cpp"]
 LIB_NAME = "libcvs_b200.so"
 
 
@@ -96,21 +98,28 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
 
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     out = PKG / ("_C" + suffix)
-    src = CSRC / "torch_ext.cpp"
+    sources = [CSRC / s for s in EXT_SOURCES]
     lib = PKG / LIB_NAME
-    if not force and not _stale(out, [src, lib] + _headers()):
+    if not force and not _stale(out, sources + [lib] + _headers()):
         return out
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    inc = [f"-I{p}" for p in cpp_extension.include_paths()] + [
+    inc = [f"-I{CSRC}"] + [f"-I{p}" for p in cpp_extension.include_paths()] + [
         f"-I{sysconfig.get_paths()['include']}",
         f"-I{_cuda_home() / 'include'}",
         f"-I{INCLUDE}",
     ]
     libdirs = [f"-L{p}" for p in cpp_extension.library_paths()]
+    flags = ["-O2", "-fPIC", "-std=c++17", "-w"] + inc + [
+        "-DTORCH_EXTENSION_NAME=_C", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_API_INCLUDE_EXTENSION_H"]
+    BUILD.mkdir(exist_ok=True)
+    objs = [BUILD / (s.stem + ".o") for s in sources]
+    jobs = [["g++"] + flags + ["-c", str(s), "-o", str(o)]
+            for s, o in zip(sources, objs) if force or _stale(o, [s] + _headers())]
+    with ThreadPoolExecutor(max_workers=max(1, len(jobs))) as ex:
+        list(ex.map(lambda c: _run(c, verbose), jobs))
     cmd = (
-        ["g++", "-O2", "-shared", "-fPIC", "-std=c++17", "-w", str(src), "-o", str(out)]
-        + inc
-        + ["-DTORCH_EXTENSION_NAME=_C", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_API_INCLUDE_EXTENSION_H"]
+        ["g++", "-shared", "-o", str(out)]
+        + [str(o) for o in objs]
         + libdirs
         + [f"-L{PKG}", "-l:" + LIB_NAME, "-Wl,-rpath,$ORIGIN"]
         + ["-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda", "-ltorch_cuda"]

@@ -1,0 +1,533 @@
+// Host side of the adapter operators' C ABI (include/cvs.h): argument contracts,
+// tile plans and tensor maps of the linear layer's products, kernel launches.
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+
+#include "cvs.h"
+#include "cvs_host.h"
+#include "cvs_kernels.h"
+
+namespace cvs {
+namespace {
+
+static_assert(CVS_MAX_NORM_WIDTH == kNormMaxWidth, "public limit");
+static_assert(CVS_LINEAR_SMALL_ROWS == kLinearSmallRows, "public limit");
+
+constexpr size_t kAlign = 256;
+size_t up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool float_type(int t) { return t == CVS_F32 || t == CVS_F16 || t == CVS_BF16; }
+
+cvs_status check_workspace(const void* ws, size_t have, size_t need) {
+  if (need == 0) return CVS_OK;
+  if (!ws || have < need || (reinterpret_cast<uintptr_t>(ws) % kAlign) != 0)
+    return fail(CVS_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required, got %zu at %p", need, have, ws);
+  return CVS_OK;
+}
+
+// ---- layer norm -----------------------------------------------------------------
+cvs_status check_norm(int dtype, int64_t rows, int d, int64_t x_stride, int weight_dtype) {
+  if (rows < 0) return fail(CVS_ERR_INVALID_ARGUMENT, "row count must be >= 0");
+  if (d < 1 || d > CVS_MAX_NORM_WIDTH)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "layer norm width must be in 1 .. %d (got %d)", CVS_MAX_NORM_WIDTH, d);
+  if (!float_type(dtype)) return fail(CVS_ERR_INVALID_ARGUMENT, "unsupported dtype %d", dtype);
+  if (weight_dtype != dtype && weight_dtype != CVS_F32)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "weight dtype must be the rows' dtype or float32");
+  if (rows > 1 && x_stride < 0) return fail(CVS_ERR_INVALID_ARGUMENT, "negative row stride");
+  return CVS_OK;
+}
+
+// ---- linear ---------------------------------------------------------------------
+cvs_status check_linear(int activation, int dtype, int64_t m, int n, int k) {
+  if (m < 0 || m >= INT_MAX) return fail(CVS_ERR_INVALID_ARGUMENT, "row count %lld out of range", (long long)m);
+  if (n < 1 || k < 1 || n > (1 << 24) || k > (1 << 24))
+    return fail(CVS_ERR_INVALID_ARGUMENT, "layer widths must be in 1 .. 2^24 (got %d x %d)", n, k);
+  if (activation < CVS_ACT_NONE || activation > CVS_ACT_SILU)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "unknown activation %d", activation);
+  if (dtype != CVS_F16 && dtype != CVS_BF16)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "linear takes float16 or bfloat16 (got dtype %d)", dtype);
+  return CVS_OK;
+}
+
+cvs_status check_operand(const void* p, int64_t stride, int64_t width, const char* name) {
+  if (!p || !aligned16(p) || stride % 8 != 0 || stride < width)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "%s must be non-null and 16-byte aligned with a row stride that is a multiple of 8 and "
+                "at least its width", name);
+  return CVS_OK;
+}
+
+// Tensor map of a half-precision matrix [rows][cols], rows `stride` elements apart,
+// in boxes of 64 columns (one 128-byte swizzled row) x box_rows rows.
+cvs_status make_half_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int64_t cols, int64_t stride,
+                         int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return fail(CVS_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r =
+      fn(map, dtype == CVS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(CVS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return CVS_OK;
+}
+
+// A product's operand: stored [mn][k] (K-major) or [k][mn] (MN-major).
+struct Operand {
+  const void* p;
+  int64_t stride;
+  bool mn_major;
+};
+
+cvs_status operand_map(CUtensorMap* map, const Operand& o, int dtype, int64_t mn, int64_t k, int box_mn) {
+  return o.mn_major ? make_half_map(map, o.p, dtype, k, mn, o.stride, 64)
+                    : make_half_map(map, o.p, dtype, mn, k, o.stride, box_mn);
+}
+
+struct Tile {
+  int cg, bn;
+  int slots(int sms) const { return sms / cg; }
+};
+constexpr Tile kTiles[3] = {{2, 256}, {1, 128}, {1, 64}};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Time of one work item in units of 128 x 64 x 64 products per SM: larger tiles
+// keep the tensor cores busier per byte of shared memory read.
+double tile_cost(const Tile& t) { return t.cg == 2 ? 4.0 : (t.bn == 128 ? 2.7 : 2.0); }
+
+// The tile shape whose rounds of work items over the SMs take least: large tiles
+// for large products, small ones where large ones would leave SMs idle.
+Tile pick_tile(int64_t m, int64_t n, int sms) {
+  Tile best = kTiles[0];
+  double best_time = 0;
+  for (const Tile& t : kTiles) {
+    const int64_t tiles = ceil_div(m, 128 * t.cg) * ceil_div(n, t.bn);
+    const double time = static_cast<double>(ceil_div(tiles, t.slots(sms))) * tile_cost(t);
+    if (best_time == 0 || time < best_time) {
+      best = t;
+      best_time = time;
+    }
+  }
+  return best;
+}
+
+void set_shape(GemmProblem* p, const Tile& t, int64_t m, int64_t n, int64_t k, int splits) {
+  p->m = static_cast<int>(m);
+  p->n = static_cast<int>(n);
+  p->tiles_m = static_cast<int>(ceil_div(m, 128 * t.cg));
+  p->tiles_n = static_cast<int>(ceil_div(n, t.bn));
+  p->kblocks = static_cast<int>(ceil_div(k, 64));
+  p->kper = static_cast<int>(ceil_div(p->kblocks, splits));
+  p->splits = static_cast<int>(ceil_div(p->kblocks, p->kper));
+  p->work = p->tiles_m * p->tiles_n * p->splits;
+}
+
+int grid_ctas(const Tile& t, int work, int sms) { return t.cg * std::max(1, std::min(t.slots(sms), work)); }
+
+// Backward: the tile shape, dw's parts along K (= rows), and the workspace.
+struct BackwardPlan {
+  Tile tile;
+  int splits;
+  int db_parts;
+  size_t dz_offset, db_offset, dw_offset, bytes;
+  int64_t dz_stride;
+};
+
+BackwardPlan plan_backward(int64_t m, int n, int k, int sms) {
+  BackwardPlan b;
+  // Both products run in one launch, with one tile shape; dw's K dimension (the
+  // rows) is cut so that its work items are about as long as dx's.
+  b.tile = pick_tile(std::max<int64_t>(m, n), k, sms);
+  const int64_t tiles = ceil_div(n, 128 * b.tile.cg) * ceil_div(k, b.tile.bn);
+  const int64_t kblocks = ceil_div(m, 64);
+  const int64_t by_length = ceil_div(kblocks, std::max<int64_t>(4, ceil_div(n, 64)));
+  const int64_t by_slots = std::max<int64_t>(1, 4 * b.tile.slots(sms) / tiles);
+  GemmProblem p{};
+  set_shape(&p, b.tile, n, k, m, static_cast<int>(std::max<int64_t>(1, std::min(by_length, by_slots))));
+  b.splits = p.splits;
+  b.db_parts = linear_dz_parts(m, n, sms);
+  b.dz_stride = (static_cast<int64_t>(n) + 7) / 8 * 8;
+  size_t at = 0;
+  b.dz_offset = at;
+  at += up(static_cast<size_t>(m) * b.dz_stride * 2);
+  b.db_offset = at;
+  at += up(static_cast<size_t>(b.db_parts) * n * 4);
+  b.dw_offset = at;
+  if (b.splits > 1) at += up(static_cast<size_t>(p.work) * b.tile.cg * 128 * b.tile.bn * 4);
+  b.bytes = at;
+  return b;
+}
+
+}  // namespace
+}  // namespace cvs
+
+using namespace cvs;
+
+extern "C" {
+
+cvs_status cvs_layer_norm(const void* x, int dtype, int64_t rows, int d, int64_t x_stride, const void* weight,
+                          const void* bias, int weight_dtype, float eps, void* y, int64_t y_stride, float* mean,
+                          float* rstd, void* stream) {
+  cvs_status st = check_norm(dtype, rows, d, x_stride, weight_dtype);
+  if (st != CVS_OK) return st;
+  if (rows == 0) return CVS_OK;
+  if (!x || !y) return fail(CVS_ERR_INVALID_ARGUMENT, "null pointer");
+  if (rows > 1 && y_stride < d) return fail(CVS_ERR_INVALID_ARGUMENT, "output row stride smaller than the width");
+  DeviceInfo dev;
+  if ((st = device_info(&dev)) != CVS_OK) return st;
+  NormArgs a{};
+  a.x = x;
+  a.weight = weight;
+  a.bias = bias;
+  a.w32 = weight_dtype == CVS_F32;
+  a.rows = rows;
+  a.d = d;
+  a.x_stride = x_stride;
+  a.eps = eps;
+  a.y = y;
+  a.y_stride = y_stride;
+  a.mean = mean;
+  a.rstd = rstd;
+  const cudaError_t e = norm_launch(a, dtype, false, dev.sms, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CVS_OK : cuda_fail(e, "layer norm launch");
+}
+
+cvs_status cvs_layer_norm_backward_workspace_size(int64_t rows, int d, size_t* bytes) {
+  if (!bytes) return fail(CVS_ERR_INVALID_ARGUMENT, "bytes must not be null");
+  *bytes = 0;
+  cvs_status st = check_norm(CVS_F32, rows, d, d, CVS_F32);
+  if (st != CVS_OK) return st;
+  if (rows == 0) return CVS_OK;
+  DeviceInfo dev;
+  if ((st = device_info(&dev)) != CVS_OK) return st;
+  *bytes = up(static_cast<size_t>(norm_backward_blocks(rows, d, dev.sms)) * 2 * d * 4);
+  return CVS_OK;
+}
+
+cvs_status cvs_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int dtype, int64_t rows, int d,
+                                   int64_t x_stride, const void* weight, int weight_dtype, const float* mean,
+                                   const float* rstd, void* dx, int64_t dx_stride, void* dweight, void* dbias,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  cvs_status st = check_norm(dtype, rows, d, x_stride, weight_dtype);
+  if (st != CVS_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const size_t ws = weight_dtype == CVS_F32 ? 4 : 2;
+  if (rows == 0) {  // sums over no rows
+    cudaError_t e = cudaSuccess;
+    if (dweight) e = cudaMemsetAsync(dweight, 0, ws * d, s);
+    if (e == cudaSuccess && dbias) e = cudaMemsetAsync(dbias, 0, ws * d, s);
+    return e == cudaSuccess ? CVS_OK : cuda_fail(e, "clearing the weights' gradients");
+  }
+  if (!dy || !x || !mean || !rstd) return fail(CVS_ERR_INVALID_ARGUMENT, "null pointer");
+  if (rows > 1 && dy_stride < 0) return fail(CVS_ERR_INVALID_ARGUMENT, "negative row stride");
+  if (dx && rows > 1 && dx_stride < d) return fail(CVS_ERR_INVALID_ARGUMENT, "gradient row stride smaller than the width");
+  if (!dx && !dweight && !dbias) return CVS_OK;
+  DeviceInfo dev;
+  if ((st = device_info(&dev)) != CVS_OK) return st;
+  const bool sums = dweight || dbias;
+  if (sums) {
+    const size_t need = up(static_cast<size_t>(norm_backward_blocks(rows, d, dev.sms)) * 2 * d * 4);
+    if ((st = check_workspace(workspace, workspace_bytes, need)) != CVS_OK) return st;
+  }
+  NormArgs a{};
+  a.x = x;
+  a.weight = weight;
+  a.w32 = weight_dtype == CVS_F32;
+  a.rows = rows;
+  a.d = d;
+  a.x_stride = x_stride;
+  a.mean = const_cast<float*>(mean);
+  a.rstd = const_cast<float*>(rstd);
+  a.dy = dy;
+  a.dy_stride = dy_stride;
+  a.dx = dx;
+  a.dx_stride = dx_stride;
+  a.dweight = dweight;
+  a.dbias = dbias;
+  a.partial = sums ? static_cast<float*>(workspace) : nullptr;
+  const cudaError_t e = norm_launch(a, dtype, true, dev.sms, s);
+  return e == cudaSuccess ? CVS_OK : cuda_fail(e, "layer norm backward launch");
+}
+
+cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
+                      const void* residual, int64_t residual_stride, int activation, int dtype, int64_t m, int n,
+                      int k, void* y, int64_t y_stride, void* z, int64_t z_stride, void* stream) {
+  cvs_status st = check_linear(activation, dtype, m, n, k);
+  if (st != CVS_OK) return st;
+  if (m == 0) return CVS_OK;
+  if (!x || !w || !y) return fail(CVS_ERR_INVALID_ARGUMENT, "null pointer");
+  if (m > 1 && y_stride < n) return fail(CVS_ERR_INVALID_ARGUMENT, "output row stride smaller than the width");
+  if (z && (!aligned16(z) || z_stride % 8 != 0 || z_stride < n))
+    return fail(CVS_ERR_INVALID_ARGUMENT, "z must be 16-byte aligned with a row stride that is a multiple of 8 and at least n");
+  if (residual && m > 1 && residual_stride < 0) return fail(CVS_ERR_INVALID_ARGUMENT, "negative row stride");
+  DeviceInfo dev;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (m <= kLinearSmallRows) {
+    if ((m > 1 && x_stride < 0) || w_stride < k)
+      return fail(CVS_ERR_INVALID_ARGUMENT, "bad row stride");
+    if ((st = device_info(&dev)) != CVS_OK) return st;
+    LinearSmallArgs a{};
+    a.x = x;
+    a.w = w;
+    a.bias = bias;
+    a.residual = residual;
+    a.out = y;
+    a.z = z;
+    a.ld_x = x_stride;
+    a.ld_w = w_stride;
+    a.ld_res = residual_stride;
+    a.ld_out = y_stride;
+    a.ld_z = z_stride;
+    a.m = static_cast<int>(m);
+    a.n = n;
+    a.k = k;
+    a.act = activation;
+    a.bf16 = dtype == CVS_BF16;
+    a.vec = aligned16(x) && aligned16(w) && x_stride % 8 == 0 && w_stride % 8 == 0 && k % 8 == 0;
+    if ((e = linear_small_launch(a, s)) != cudaSuccess) return cuda_fail(e, "linear launch");
+    return CVS_OK;
+  }
+  if ((st = check_operand(x, x_stride, k, "x")) != CVS_OK) return st;
+  if ((st = check_operand(w, w_stride, k, "w")) != CVS_OK) return st;
+  if ((st = device_info(&dev)) != CVS_OK) return st;
+  const Tile t = pick_tile(m, n, dev.sms);
+  CUtensorMap maps[4];
+  if ((st = operand_map(&maps[0], {x, x_stride, false}, dtype, m, k, 128)) != CVS_OK) return st;
+  if ((st = operand_map(&maps[1], {w, w_stride, false}, dtype, n, k, t.bn / t.cg)) != CVS_OK) return st;
+  maps[2] = maps[0];
+  maps[3] = maps[1];
+  GemmArgs a{};
+  GemmProblem& p = a.p[0];
+  set_shape(&p, t, m, n, k, 1);
+  p.act = activation;
+  p.out = y;
+  p.ld_out = y_stride;
+  p.vec_out = aligned16(y) && y_stride % 8 == 0;
+  p.bias = bias;
+  p.residual = residual;
+  p.ld_res = residual_stride;
+  p.vec_res = aligned16(residual) && residual_stride % 8 == 0;
+  p.z = z;
+  p.ld_z = z_stride;
+  a.bf16 = dtype == CVS_BF16;
+  a.err = dev.err;
+  e = gemm_launch(t.cg, t.bn, maps, a, grid_ctas(t, p.work, dev.sms), s);
+  return e == cudaSuccess ? CVS_OK : cuda_fail(e, "linear launch");
+}
+
+cvs_status cvs_linear_backward_workspace_size(int activation, int64_t m, int n, int k, size_t* bytes) {
+  if (!bytes) return fail(CVS_ERR_INVALID_ARGUMENT, "bytes must not be null");
+  *bytes = 0;
+  cvs_status st = check_linear(activation, CVS_F16, m, n, k);
+  if (st != CVS_OK) return st;
+  if (m == 0) return CVS_OK;
+  DeviceInfo dev;
+  if ((st = device_info(&dev)) != CVS_OK) return st;
+  *bytes = plan_backward(m, n, k, dev.sms).bytes;
+  return CVS_OK;
+}
+
+cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w,
+                               int64_t w_stride, const void* z, int64_t z_stride, int activation, int dtype,
+                               int64_t m, int n, int k, void* dx, int64_t dx_stride, void* dw, int64_t dw_stride,
+                               void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+  cvs_status st = check_linear(activation, dtype, m, n, k);
+  if (st != CVS_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (dw && n > 1 && dw_stride < k) return fail(CVS_ERR_INVALID_ARGUMENT, "dw row stride smaller than its width");
+  if (m == 0) {  // sums over no rows
+    if (dw) e = cudaMemset2DAsync(dw, static_cast<size_t>(std::max<int64_t>(dw_stride, k)) * 2, 0, static_cast<size_t>(k) * 2, n, s);
+    if (e == cudaSuccess && dbias) e = cudaMemsetAsync(dbias, 0, static_cast<size_t>(n) * 2, s);
+    return e == cudaSuccess ? CVS_OK : cuda_fail(e, "clearing the weights' gradients");
+  }
+  if (!dx && !dw && !dbias) return CVS_OK;
+  if (!dy) return fail(CVS_ERR_INVALID_ARGUMENT, "null pointer");
+  if (m > 1 && dy_stride < 0) return fail(CVS_ERR_INVALID_ARGUMENT, "negative row stride");
+  if (dx && m > 1 && dx_stride < k) return fail(CVS_ERR_INVALID_ARGUMENT, "dx row stride smaller than its width");
+  if (dw && (st = check_operand(x, x_stride, k, "x")) != CVS_OK) return st;
+  if (dx && (st = check_operand(w, w_stride, k, "w")) != CVS_OK) return st;
+  const bool act = activation != CVS_ACT_NONE;
+  if (act && (!z || !aligned16(z) || z_stride % 8 != 0 || z_stride < n))
+    return fail(CVS_ERR_INVALID_ARGUMENT, "z must be 16-byte aligned with a row stride that is a multiple of 8 and at least n");
+  DeviceInfo dev;
+  if ((st = device_info(&dev)) != CVS_OK) return st;
+  const BackwardPlan plan = plan_backward(m, n, k, dev.sms);
+  if ((st = check_workspace(workspace, workspace_bytes, plan.bytes)) != CVS_OK) return st;
+  char* base = static_cast<char*>(workspace);
+  const bool bf16 = dtype == CVS_BF16;
+  const bool dy_tiles = aligned16(dy) && dy_stride % 8 == 0 && dy_stride >= n;  // TMA can read dy itself
+  Operand dz{dy, dy_stride, false};
+  if (act || !dy_tiles) dz = {base + plan.dz_offset, plan.dz_stride, false};
+  if (act || dbias || (!dy_tiles && (dx || dw))) {
+    LinearDzArgs a{};
+    a.dy = dy;
+    a.ld_dy = dy_stride;
+    a.vec_dy = aligned16(dy) && dy_stride % 8 == 0;
+    a.z = act ? z : nullptr;
+    a.ld_z = z_stride;
+    a.dz = dz.p == dy || !(dx || dw) ? nullptr : const_cast<void*>(dz.p);
+    a.ld_dz = plan.dz_stride;
+    a.partial = dbias ? reinterpret_cast<float*>(base + plan.db_offset) : nullptr;
+    a.m = m;
+    a.n = n;
+    a.act = activation;
+    a.bf16 = bf16;
+    if ((e = linear_dz_launch(a, plan.db_parts, s)) != cudaSuccess) return cuda_fail(e, "linear backward launch");
+  }
+  const Tile& t = plan.tile;
+  if (dx || dw) {
+    CUtensorMap maps[4];
+    GemmArgs a{};
+    a.bf16 = bf16;
+    a.err = dev.err;
+    int i = 0;
+    if (dw) {  // dw[n][k] = dz^T x: both operands have K (the rows) as their outer dimension
+      GemmProblem& p = a.p[i];
+      set_shape(&p, t, n, k, m, plan.splits);
+      p.a_mn = p.b_mn = 1;
+      p.out = dw;
+      p.ld_out = dw_stride;
+      p.vec_out = aligned16(dw) && dw_stride % 8 == 0;
+      p.partial = p.splits > 1 ? reinterpret_cast<float*>(base + plan.dw_offset) : nullptr;
+      if ((st = operand_map(&maps[2 * i], {dz.p, dz.stride, true}, dtype, n, m, 64)) != CVS_OK) return st;
+      if ((st = operand_map(&maps[2 * i + 1], {x, x_stride, true}, dtype, k, m, 64)) != CVS_OK) return st;
+      ++i;
+    }
+    if (dx) {  // dx[m][k] = dz w: w has K (its n rows) as its outer dimension
+      GemmProblem& p = a.p[i];
+      set_shape(&p, t, m, k, n, 1);
+      p.b_mn = 1;
+      p.out = dx;
+      p.ld_out = dx_stride;
+      p.vec_out = aligned16(dx) && dx_stride % 8 == 0;
+      if ((st = operand_map(&maps[2 * i], dz, dtype, m, n, 128)) != CVS_OK) return st;
+      if ((st = operand_map(&maps[2 * i + 1], {w, w_stride, true}, dtype, k, n, 64)) != CVS_OK) return st;
+      ++i;
+    }
+    if (i == 1) {
+      maps[2] = maps[0];
+      maps[3] = maps[1];
+    }
+    const int work = a.p[0].work + a.p[1].work;
+    if ((e = gemm_launch(t.cg, t.bn, maps, a, grid_ctas(t, work, dev.sms), s)) != cudaSuccess)
+      return cuda_fail(e, "linear backward launch");
+  }
+  LinearFinishArgs f{};
+  f.db_partial = reinterpret_cast<const float*>(base + plan.db_offset);
+  f.db_parts = plan.db_parts;
+  f.db_blocks = dbias ? (n + 31) / 32 : 0;
+  f.dbias = dbias;
+  f.dw_partial = dw && plan.splits > 1 ? reinterpret_cast<const float*>(base + plan.dw_offset) : nullptr;
+  f.splits = plan.splits;
+  f.tiles_m = static_cast<int>(ceil_div(n, 128 * t.cg));
+  f.tiles_n = static_cast<int>(ceil_div(k, t.bn));
+  f.cg = t.cg;
+  f.bn = t.bn;
+  f.dw = dw;
+  f.ld_dw = dw_stride;
+  f.n = n;
+  f.k = k;
+  f.bf16 = bf16;
+  if ((e = linear_finish_launch(f, s)) != cudaSuccess) return cuda_fail(e, "linear backward launch");
+  return CVS_OK;
+}
+
+cvs_status cvs_preference_loss_workspace_size(int64_t b, int r, size_t* bytes) {
+  if (!bytes) return fail(CVS_ERR_INVALID_ARGUMENT, "bytes must not be null");
+  *bytes = 0;
+  if (b < 0 || b >= INT_MAX) return fail(CVS_ERR_INVALID_ARGUMENT, "query count out of range");
+  if (r < 1) return fail(CVS_ERR_INVALID_ARGUMENT, "at least one rejected row per query");
+  if (b == 0) return CVS_OK;
+  DeviceInfo dev;
+  const cvs_status st = device_info(&dev);
+  if (st != CVS_OK) return st;
+  *bytes = up(static_cast<size_t>(preference_blocks(b, r, dev.sms)) * 8);
+  return CVS_OK;
+}
+
+cvs_status cvs_preference_loss(const void* q, int q_dtype, int64_t q_stride, const void* ref, int ref_dtype,
+                               int64_t ref_stride, int64_t b, int d, int cosine, const void* x_f16, int64_t n,
+                               int d_pad, const int64_t* chosen, const int64_t* rejected, int64_t rejected_stride,
+                               int r, float scale, float label_smoothing, int mean, float* loss, float* weight,
+                               float* margins, float* grad, int64_t grad_stride, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  if (b < 0 || b >= INT_MAX) return fail(CVS_ERR_INVALID_ARGUMENT, "query count %lld out of range", (long long)b);
+  if (r < 1) return fail(CVS_ERR_INVALID_ARGUMENT, "at least one rejected row per query");
+  if (n < 1 || n >= INT_MAX)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "corpus must have 1 .. 2^31-1 rows (got %lld)", (long long)n);
+  if (d_pad < CVS_PAD || d_pad % CVS_PAD != 0 || d_pad > 2048)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "corpus width must be a multiple of 64 up to 2048 (got %d)", d_pad);
+  if (d < 1 || d > d_pad) return fail(CVS_ERR_INVALID_ARGUMENT, "query width %d exceeds the corpus width %d", d, d_pad);
+  if (!float_type(q_dtype) || (ref && !float_type(ref_dtype)))
+    return fail(CVS_ERR_INVALID_ARGUMENT, "queries must be float32, float16 or bfloat16");
+  if (!(label_smoothing >= 0.f && label_smoothing <= 1.f))
+    return fail(CVS_ERR_INVALID_ARGUMENT, "label smoothing must be in 0 .. 1");
+  if (!x_f16 || !aligned16(x_f16)) return fail(CVS_ERR_INVALID_ARGUMENT, "corpus must be a non-null 16-byte aligned pointer");
+  if (!loss || !weight) return fail(CVS_ERR_INVALID_ARGUMENT, "null output pointer");
+  if (b > 0 && (!q || !chosen || !rejected || !margins)) return fail(CVS_ERR_INVALID_ARGUMENT, "null pointer");
+  if (b > 1 && (q_stride < 0 || (ref && ref_stride < 0) || rejected_stride < 0))
+    return fail(CVS_ERR_INVALID_ARGUMENT, "negative row stride");
+  if (grad && (!aligned16(grad) || grad_stride % 8 != 0 || grad_stride < d))
+    return fail(CVS_ERR_INVALID_ARGUMENT, "grad must be 16-byte aligned with a row stride that is a multiple of 8 and at least d");
+  DeviceInfo dev;
+  cvs_status st = device_info(&dev);
+  if (st != CVS_OK) return st;
+  const size_t need = b == 0 ? 0 : up(static_cast<size_t>(preference_blocks(b, r, dev.sms)) * 8);
+  if ((st = check_workspace(workspace, workspace_bytes, need)) != CVS_OK) return st;
+  const auto vec = [d](const void* p, int dtype, int64_t stride) {
+    return d % 8 == 0 && aligned16(p) && (stride * (dtype == CVS_F32 ? 4 : 2)) % 16 == 0;
+  };
+  PreferenceArgs a{};
+  a.q = q;
+  a.ref = ref;
+  a.q_dtype = q_dtype;
+  a.ref_dtype = ref_dtype;
+  a.q_stride = q_stride;
+  a.ref_stride = ref_stride;
+  a.q_vec = vec(q, q_dtype, q_stride);
+  a.ref_vec = ref && vec(ref, ref_dtype, ref_stride);
+  a.cosine = cosine;
+  a.x = static_cast<const __half*>(x_f16);
+  a.n = n;
+  a.d = d;
+  a.d_pad = d_pad;
+  a.chosen = reinterpret_cast<const long long*>(chosen);
+  a.rejected = reinterpret_cast<const long long*>(rejected);
+  a.rejected_stride = rejected_stride;
+  a.b = b;
+  a.r = r;
+  a.scale = scale;
+  a.smoothing = label_smoothing;
+  a.margins = margins;
+  a.grad = grad;
+  a.grad_stride = grad_stride;
+  a.partial = static_cast<float2*>(workspace);
+  const cudaError_t e = preference_launch(a, mean, loss, weight, dev.sms, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CVS_OK : cuda_fail(e, "preference loss launch");
+}
+
+cvs_status cvs_preference_grad(const float* grad, int64_t grad_stride, int64_t b, int d, const float* weight,
+                               const float* upstream, int dtype, void* dq, void* stream) {
+  if (b < 0 || b >= INT_MAX) return fail(CVS_ERR_INVALID_ARGUMENT, "query count out of range");
+  if (b == 0) return CVS_OK;
+  if (d < 1 || grad_stride < d || grad_stride % 8 != 0)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "grad's row stride must be a multiple of 8 and at least d");
+  if (!grad || !aligned16(grad) || !weight || !upstream || !dq)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "null or misaligned pointer");
+  if (!float_type(dtype)) return fail(CVS_ERR_INVALID_ARGUMENT, "unsupported dtype %d", dtype);
+  DeviceInfo dev;
+  const cvs_status st = device_info(&dev);
+  if (st != CVS_OK) return st;
+  const cudaError_t e = preference_grad_launch(grad, grad_stride, b, d, weight, upstream, dtype, dq, dev.sms,
+                                               static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CVS_OK : cuda_fail(e, "preference gradient launch");
+}
+
+}  // extern "C"

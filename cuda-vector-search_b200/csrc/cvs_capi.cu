@@ -18,6 +18,7 @@
 #include <unordered_map>
 
 #include "cvs.h"
+#include "cvs_host.h"
 #include "cvs_kernels.h"
 
 namespace cvs {
@@ -28,7 +29,8 @@ __device__ int g_device_error;  // one word per device; written by kernels on a 
 thread_local std::string g_last_error;
 thread_local int64_t g_stall_cycles = 0;  // armed failure-path test (cvs_debug_stall_next_search)
 
-cvs_status fail(cvs_status s, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+}  // namespace
+
 cvs_status fail(cvs_status s, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -43,19 +45,16 @@ cvs_status cuda_fail(cudaError_t e, const char* what) {
   return fail(CVS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-struct DeviceInfo {
-  int sms = 0;
-  int major = 0;
-  int minor = 0;
-  int* err = nullptr;  // device address of g_device_error
-};
+namespace {
 
 std::mutex g_mu;
 std::unordered_map<int, DeviceInfo> g_devices;
 cudaEvent_t g_prof_start = nullptr;
 cudaEvent_t g_prof_stop = nullptr;
 
-cvs_status device_info(DeviceInfo* out, int* dev_out = nullptr) {
+}  // namespace
+
+cvs_status device_info(DeviceInfo* out, int* dev_out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
@@ -94,6 +93,8 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   });
   return fn;
 }
+
+namespace {
 
 // 2-D fp16 tensor [rows][cols], boxes of 64 columns x box_rows rows, 128-byte swizzle.
 cvs_status make_map(CUtensorMap* m, const void* base, int64_t rows, int cols, int box_rows) {

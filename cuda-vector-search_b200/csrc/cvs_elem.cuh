@@ -1,0 +1,103 @@
+// Element access shared by the adapter kernels (layer norm, linear, preference
+// loss): eight consecutive or eight strided elements of a row as fp32, from
+// fp32, fp16 or bf16 storage.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+
+namespace cvs {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Eight elements as stored: 16 bytes (halves) or 32 bytes (fp32).
+template <class T>
+struct alignas(16) Raw8 {
+  T v[8];
+};
+
+template <class T>
+__device__ __forceinline__ Raw8<T> zero8() {
+  Raw8<T> r;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) r.v[t] = from_f32<T>(0.f);
+  return r;
+}
+
+// p must be 16-byte aligned.
+template <class T>
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+  Raw8<T> r;
+  const uint4* s = reinterpret_cast<const uint4*>(p);
+  uint4* d = reinterpret_cast<uint4*>(&r);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i) d[i] = s[i];
+  return r;
+}
+
+template <class T>
+__device__ __forceinline__ void store8(T* p, const Raw8<T>& r) {
+  const uint4* s = reinterpret_cast<const uint4*>(&r);
+  uint4* d = reinterpret_cast<uint4*>(p);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i) d[i] = s[i];
+}
+
+// The j-th group of eight columns that thread `tid` of `threads` owns in a row
+// of d columns. Aligned rows (VEC): eight consecutive columns, one 16-byte (or
+// two) access; d is a multiple of 8. Otherwise eight single columns `threads`
+// apart, so that a warp's scalar accesses still cover consecutive elements.
+template <bool VEC>
+struct Cols {
+  static __device__ __forceinline__ int at(int tid, int threads, int j, int t) {
+    return VEC ? (tid + threads * j) * 8 + t : tid + threads * (8 * j + t);
+  }
+  template <class T>
+  static __device__ __forceinline__ Raw8<T> load(const T* row, int d, int tid, int threads, int j) {
+    if constexpr (VEC) {
+      const int c = (tid + threads * j) * 8;
+      return c < d ? load8(row + c) : zero8<T>();
+    } else {
+      Raw8<T> r = zero8<T>();
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const int c = at(tid, threads, j, t);
+        if (c < d) r.v[t] = row[c];
+      }
+      return r;
+    }
+  }
+  template <class T>
+  static __device__ __forceinline__ void store(T* row, int d, int tid, int threads, int j, const Raw8<T>& r) {
+    if constexpr (VEC) {
+      const int c = (tid + threads * j) * 8;
+      if (c < d) store8(row + c, r);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const int c = at(tid, threads, j, t);
+        if (c < d) row[c] = r.v[t];
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+
+}  // namespace cvs

@@ -195,4 +195,132 @@ cudaError_t ingest_launch(const void* src, int src_dtype, long long n, int d, lo
                           int d_pad, int cosine, __half* dst, int num_sms, cudaStream_t stream,
                           uint32_t* clear = nullptr, size_t clear_words = 0, long long rows_pad = 0);
 
+// ---- layer norm -------------------------------------------------------------
+constexpr int kNormMaxWidth = 8192;
+
+struct NormArgs {
+  const void* x;       // [rows][d], rows x_stride elements apart
+  const void* weight;  // [d] or null (ones); fp32 if w32, else the rows' type
+  const void* bias;    // [d] or null (zeros), same type as weight
+  int w32;
+  long long rows;
+  int d;
+  long long x_stride;
+  float eps;
+  void* y;             // forward result
+  long long y_stride;
+  float* mean;         // [rows]: forward writes them (or null), backward reads them
+  float* rstd;
+  const void* dy;      // backward only
+  long long dy_stride;
+  void* dx;            // null: not wanted
+  long long dx_stride;
+  void* dweight;       // null: not wanted
+  void* dbias;
+  float* partial;      // [blocks][2][d] or null when neither dweight nor dbias is wanted
+};
+// Blocks of the backward kernel, each with its own row of `partial`.
+int norm_backward_blocks(long long rows, int d, int num_sms);
+cudaError_t norm_launch(const NormArgs& a, int dtype, bool backward, int num_sms, cudaStream_t stream);
+
+// ---- linear layer -------------------------------------------------------------
+enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
+constexpr int kLinearSmallRows = 8;  // rows up to which the weights are streamed by CUDA cores
+
+// One product out[m][n] = A B^T over kblocks slices of 64 along K, cut into
+// `splits` parts of kper slices. All pointers hold halves of the call's type
+// except z (fp16) and partial (fp32).
+struct GemmProblem {
+  int work;              // work items: tiles_m * tiles_n * splits (0: no such product)
+  int tiles_m, tiles_n;
+  int splits, kblocks, kper;
+  int m, n;
+  int a_mn, b_mn;        // operand stored with K as its outer dimension
+  int act;
+  void* out;
+  long long ld_out;
+  const void* bias;      // [n] or null
+  const void* residual;  // [m][n] or null
+  long long ld_res;
+  void* z;               // pre-activation, fp16, rows 16-byte aligned, or null
+  long long ld_z;
+  int vec_out, vec_res;  // rows 16-byte aligned
+  float* partial;        // splits > 1: fp32 parts instead of all of the above
+};
+struct GemmArgs {
+  GemmProblem p[2];
+  int bf16;
+  int* err;
+};
+// Tile shapes: cg CTAs (128 rows each) x bn columns. maps: A and B of both products.
+cudaError_t gemm_launch(int cg, int bn, const CUtensorMap (&maps)[4], const GemmArgs& a, int ctas, cudaStream_t stream);
+
+struct LinearSmallArgs {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* residual;
+  void* out;
+  void* z;
+  long long ld_x, ld_w, ld_res, ld_out, ld_z;
+  int m, n, k;
+  int act, bf16;
+  int vec;  // x and w rows 16-byte aligned and k a multiple of 8
+};
+cudaError_t linear_small_launch(const LinearSmallArgs& a, cudaStream_t stream);
+
+struct LinearDzArgs {
+  const void* dy;
+  const void* z;     // null: no activation
+  void* dz;          // null: dy is used as it is
+  float* partial;    // [parts][n] column sums, or null
+  long long ld_dy, ld_z, ld_dz;
+  long long m;
+  int n;
+  int act, bf16, vec_dy;
+};
+int linear_dz_parts(long long m, int n, int num_sms);
+cudaError_t linear_dz_launch(const LinearDzArgs& a, int parts, cudaStream_t stream);
+
+struct LinearFinishArgs {
+  const float* db_partial;
+  int db_parts, db_blocks;  // db_blocks: ceil(n / 32), 0 when dbias is not wanted
+  void* dbias;
+  const float* dw_partial;  // null when dw was written by the product itself
+  int splits, tiles_m, tiles_n, cg, bn;
+  void* dw;
+  long long ld_dw;
+  int n, k;                 // dw is [n][k]
+  int bf16;
+};
+cudaError_t linear_finish_launch(const LinearFinishArgs& a, cudaStream_t stream);
+
+// ---- preference loss ------------------------------------------------------------
+struct PreferenceArgs {
+  const void* q;            // [b][d]
+  const void* ref;          // [b][d] or null
+  int q_dtype, ref_dtype;
+  long long q_stride, ref_stride;
+  int q_vec, ref_vec;       // rows 16-byte aligned and d a multiple of 8
+  int cosine;
+  const __half* x;          // [n][d_pad]
+  long long n;
+  int d, d_pad;
+  const long long* chosen;  // [b]
+  const long long* rejected;  // [b][r], rows rejected_stride apart
+  long long rejected_stride;
+  long long b;
+  int r;
+  float scale, smoothing;
+  float* margins;           // [b][r]
+  float* grad;              // [b][grad_stride] sums of the loss's gradient, or null
+  long long grad_stride;    // d rounded up to a multiple of 8
+  float2* partial;          // [blocks] (loss, pairs)
+  int warps_per_query;      // set by preference_launch
+};
+int preference_blocks(long long b, int r, int num_sms);
+cudaError_t preference_launch(PreferenceArgs a, int mean, float* loss, float* weight, int num_sms, cudaStream_t stream);
+cudaError_t preference_grad_launch(const float* grad, long long grad_stride, long long b, int d, const float* weight,
+                                   const float* upstream, int q_dtype, void* dq, int num_sms, cudaStream_t stream);
+
 }  // namespace cvs

@@ -2,7 +2,8 @@
 // reference's extension module functions with the same names and arguments:
 //   scores(q, x, out_fp32=True)                 cuda_vector_search/csrc/kernels.cu:472-497,588
 //   fused_topk(q, x, k, bq=0, chunks=0)         cuda_vector_search/csrc/kernels.cu:501-582,590
-// plus the ingest / merge / diagnostics entry points this build adds. Contract
+// plus the ingest / merge / diagnostics entry points this build adds and, in
+// torch_adapter.cpp, the query adapter's differentiable operators. Contract
 // violations raise RuntimeError through TORCH_CHECK, as the reference's
 // check_matrix / check_pair do (kernels.cu:451-470). Everything runs on the
 // current CUDA stream of the input's device, with no host synchronisation.
@@ -14,6 +15,7 @@
 #include <vector>
 
 #include "cvs.h"
+#include "torch_adapter.h"
 
 namespace {
 
@@ -263,6 +265,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("src"), py::arg("dst"), py::arg("cosine"));
   m.def("merge_lists", &merge_lists, "Merge [lists, b, len] result lists into the best k",
         py::arg("v"), py::arg("i"), py::arg("k"));
+  cvs_torch::bind_adapter(m);
   m.def("poll_device_error", &poll_device_error, "Read and clear the device error word",
         py::arg("device"));
   m.def("set_profile_events", &set_profile_events, "Record events around the search kernel",

@@ -254,8 +254,18 @@ class Index:
         return _ingest(self._query_tensor(queries), self.device, self.metric == "cosine")
 
     # -- search -------------------------------------------------------------
-    def search(self, queries, k: int = 10, method: str = "auto"):
+    def _adapt(self, queries, adapter):
+        """The queries as ``adapter`` maps them (no gradients are kept)."""
+        q = self._query_tensor(queries)
+        with torch.no_grad(), torch.cuda.device(self.device):
+            out = adapter(q if q.device == self.device else q.to(self.device, non_blocking=q.is_pinned()))
+        return out
+
+    def search(self, queries, k: int = 10, method: str = "auto", adapter=None):
         """Return (scores [b, k] float32, ids [b, k] int64), best first.
+
+        adapter: an ``Adapter`` (or any callable on a [b, d] device tensor) that
+        maps the queries before they are compared with the corpus.
 
         method:
             "fused"   - tcgen05 (or GEMV for b = 1, and b <= 8 on small corpora) scores + top-k
@@ -273,6 +283,8 @@ class Index:
         if method == "auto":
             method = "fused" if k <= MAX_FUSED_K else "twopass"
         mod = _ext.load()
+        if adapter is not None:
+            queries = self._adapt(queries, adapter)
         if method == "fused":
             if k > MAX_FUSED_K:
                 self._query_tensor(queries)  # the reference reports bad queries first
@@ -293,6 +305,45 @@ class Index:
         """Full [b, n] score matrix from the tcgen05 score kernel."""
         q = self._prep_queries(queries)
         return _ext.load().scores(q, self._x, fp32)
+
+    # -- training -----------------------------------------------------------
+    def _ids(self, ids) -> torch.Tensor:
+        t = _to_tensor(ids)
+        return t if t.device == self.device else t.to(self.device, non_blocking=t.is_pinned())
+
+    def preference_loss(self, queries, chosen, rejected, reference=None, scale: float = 1.0,
+                        label_smoothing: float = 0.0, reduction: str = "mean", return_margins: bool = False):
+        """Preference loss of (adapted) queries over rows of this index.
+
+        For each query, ``chosen`` names the row that was preferred and ``rejected``
+        one row or several that were passed over. With scores s_i = scale * u . x_i
+        (u the query, L2-normalised for cosine) and the choice p(i) = softmax_i(s_i),
+        the log ratio of a pair against the ``reference`` query (usually the query
+        before adaptation; taken as a constant) is
+        m = scale * (u - u_ref) . (x_chosen - x_rejected), and the loss is
+        -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m).
+
+        Args:
+            queries: [b, d] float32, float16 or bfloat16 on the index device; the
+                loss is differentiable with respect to them.
+            chosen: [b] int64 row ids. rejected: [b] or [b, r] int64 row ids. Ids
+                below 0 mark absent rows: their pairs have margin 0 and do not
+                count. An id that is not a row of the index gives NaN.
+            reference: [b, d], or None for zero (plain pairwise ranking).
+            reduction: "mean" (over the pairs present; 0 when there are none) or "sum".
+            return_margins: also return the margins m, [b, r] float32 without
+                gradient; the share of positive ones is the ranking accuracy.
+        """
+        if reduction not in ("mean", "sum"):
+            raise ValueError("reduction must be 'mean' or 'sum'")
+        q = self._query_tensor(queries)
+        rejected = self._ids(rejected)
+        if rejected.dim() == 1:
+            rejected = rejected[:, None]
+        loss, margins = _ext.load().preference_loss(
+            q, reference, self._ids(chosen), rejected, self._x, self.metric == "cosine", float(scale),
+            float(label_smoothing), reduction == "mean")
+        return (loss, margins) if return_margins else loss
 
     # -- persistence --------------------------------------------------------
     def save(self, path) -> None:

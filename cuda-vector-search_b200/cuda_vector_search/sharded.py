@@ -233,13 +233,24 @@ class ShardedIndex:
 
         return _cached(self._buffers, (b, k), make)
 
-    def search(self, queries, k: int = 10):
+    def _adapt(self, queries, adapter):
+        if self.local is not None:
+            return self.local._adapt(queries, adapter)
+        with torch.no_grad():
+            q = _to_tensor(queries)
+            return adapter((q[None] if q.dim() == 1 else q).to(self.ops.device))
+
+    def search(self, queries, k: int = 10, adapter=None):
+        """(scores [b, k] f32, global ids [b, k] i64), best first, on every rank.
+        ``adapter`` maps the queries first, as in ``Index.search``."""
         k = int(k)
         if k < 1:
             raise ValueError("k must be >= 1")
         k = min(k, self.n_total)
         if k > MAX_FUSED_K:
             raise ValueError(f"sharded search supports k <= {MAX_FUSED_K}")
+        if adapter is not None:  # every rank maps the same queries (with the same adapter)
+            queries = self._adapt(queries, adapter)
         ev = self.phase_events
         if ev is not None:
             ev[0].record()

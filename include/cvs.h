@@ -193,6 +193,103 @@ cvs_status cvs_debug_stall_next_search(int64_t wait_cycles);
  */
 cvs_status cvs_set_profile_events(void* start_event, void* stop_event);
 
+/* ---------------------------------------------------------------------------
+ * Query adapter: the operators of a small network in front of the index, and
+ * the loss that trains it against a fixed corpus. No counterpart in the
+ * reference. Matrices are row-major with rows `*_stride` elements apart;
+ * `dtype` is CVS_F32, CVS_F16 or CVS_BF16 unless a function says less. All sums
+ * are fp32, and every result is rounded once. Results do not depend on the run:
+ * sums over rows are taken in a fixed order.
+ * ------------------------------------------------------------------------- */
+
+#define CVS_MAX_NORM_WIDTH 8192  /* columns of a layer norm */
+#define CVS_LINEAR_SMALL_ROWS 8  /* rows up to which cvs_linear takes operands of any alignment */
+
+typedef enum cvs_activation {
+  CVS_ACT_NONE = 0,
+  CVS_ACT_RELU = 1,
+  CVS_ACT_GELU = 2, /* z Phi(z), with the normal distribution function itself */
+  CVS_ACT_SILU = 3
+} cvs_activation;
+
+/*
+ * y = (x - mean) * rstd * weight + bias per row, rstd = 1 / sqrt(variance + eps).
+ * weight, bias: [d] of weight_dtype (dtype or CVS_F32), or NULL (ones / zeros).
+ * mean, rstd: [rows] fp32, written for the backward pass unless NULL.
+ */
+cvs_status cvs_layer_norm(const void* x, int dtype, int64_t rows, int d, int64_t x_stride, const void* weight,
+                          const void* bias, int weight_dtype, float eps, void* y, int64_t y_stride, float* mean,
+                          float* rstd, void* stream);
+
+/* Bytes of workspace cvs_layer_norm_backward needs when dweight or dbias is asked for. */
+cvs_status cvs_layer_norm_backward_workspace_size(int64_t rows, int d, size_t* bytes);
+
+/*
+ * Gradients of cvs_layer_norm from dy and the forward pass's x, mean and rstd.
+ * dx [rows][d] of dtype, dweight and dbias [d] of weight_dtype; each may be NULL
+ * (not wanted). workspace: 256-byte aligned.
+ */
+cvs_status cvs_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int dtype, int64_t rows, int d,
+                                   int64_t x_stride, const void* weight, int weight_dtype, const float* mean,
+                                   const float* rstd, void* dx, int64_t dx_stride, void* dweight, void* dbias,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * y[m][n] = act(x[m][k] . w[n][k]^T + bias) + residual, dtype CVS_F16 or CVS_BF16
+ * for every operand. bias [n] and residual [m][n] may be NULL. z, unless NULL,
+ * receives x . w^T + bias as fp16 (also for CVS_BF16) for cvs_linear_backward:
+ * 16-byte aligned, z_stride a multiple of 8.
+ * x and w: 16-byte aligned with strides a multiple of 8 unless m is at most
+ * CVS_LINEAR_SMALL_ROWS; y, bias and residual may have any alignment.
+ */
+cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
+                      const void* residual, int64_t residual_stride, int activation, int dtype, int64_t m, int n,
+                      int k, void* y, int64_t y_stride, void* z, int64_t z_stride, void* stream);
+
+/* Bytes of workspace cvs_linear_backward needs. */
+cvs_status cvs_linear_backward_workspace_size(int activation, int64_t m, int n, int k, size_t* bytes);
+
+/*
+ * Gradients of cvs_linear: dx [m][k], dw [n][k], dbias [n], each of dtype and each
+ * NULL when not wanted. z: as written by cvs_linear (not read for CVS_ACT_NONE).
+ * The residual's gradient is dy. x and w: 16-byte aligned with strides a multiple
+ * of 8; dy, dx, dw and dbias may have any alignment. workspace: 256-byte aligned.
+ */
+cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w,
+                               int64_t w_stride, const void* z, int64_t z_stride, int activation, int dtype,
+                               int64_t m, int n, int k, void* dx, int64_t dx_stride, void* dw, int64_t dw_stride,
+                               void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace cvs_preference_loss needs. */
+cvs_status cvs_preference_loss_workspace_size(int64_t b, int r, size_t* bytes);
+
+/*
+ * Preference loss of b queries over rows of the corpus x [n][d_pad] (fp16, as the
+ * index stores it): for each query a chosen row and r rejected rows, with
+ *   margin = scale * (u - u_ref) . (x[chosen] - x[rejected]),
+ *   loss = (1 - label_smoothing) softplus(-margin) + label_smoothing softplus(margin),
+ * u the query (cosine != 0: divided by max(||q||_2, 1e-12)), u_ref the reference
+ * query likewise (ref NULL: zero). Ids below 0 mark absent rows: their pairs have
+ * margin 0 and do not count. An id of n or more gives NaN.
+ *   loss: the sum over pairs, divided by their number (at least 1) when mean != 0.
+ *   weight: that divisor's inverse (1 for a sum).
+ *   margins [b][r]: fp32.
+ *   grad, unless NULL: [b][grad_stride] fp32, 16-byte aligned, grad_stride a
+ *   multiple of 8 and at least d: the gradient of the undivided sum with respect to
+ *   the queries, for cvs_preference_grad.
+ * q and ref: any alignment. workspace: 256-byte aligned.
+ */
+cvs_status cvs_preference_loss(const void* q, int q_dtype, int64_t q_stride, const void* ref, int ref_dtype,
+                               int64_t ref_stride, int64_t b, int d, int cosine, const void* x_f16, int64_t n,
+                               int d_pad, const int64_t* chosen, const int64_t* rejected, int64_t rejected_stride,
+                               int r, float scale, float label_smoothing, int mean, float* loss, float* weight,
+                               float* margins, float* grad, int64_t grad_stride, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* dq[b][d] (dense, of dtype) = grad * weight[0] * upstream[0]; upstream: fp32 device scalar. */
+cvs_status cvs_preference_grad(const float* grad, int64_t grad_stride, int64_t b, int d, const float* weight,
+                               const float* upstream, int dtype, void* dq, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
