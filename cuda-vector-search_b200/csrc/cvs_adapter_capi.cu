@@ -88,6 +88,14 @@ cvs_status operand_map(CUtensorMap* map, const Operand& o, int dtype, int64_t mn
                     : make_half_map(map, o.p, dtype, mn, k, o.stride, box_mn);
 }
 
+// Rows a tensor map can describe, and the map of what the epilogue moves.
+bool mappable(const void* p, int64_t stride, int64_t width) {
+  return p && aligned16(p) && stride % 8 == 0 && stride >= width;
+}
+cvs_status block_map(CUtensorMap* map, const void* p, int dtype, int64_t rows, int64_t cols, int64_t stride) {
+  return make_half_map(map, p, dtype, rows, cols, stride, 32);
+}
+
 struct Tile {
   int cg, bn;
   int slots(int sms) const { return sms / cg; }
@@ -140,15 +148,38 @@ struct BackwardPlan {
 
 BackwardPlan plan_backward(int64_t m, int n, int k, int sms) {
   BackwardPlan b;
-  // Both products run in one launch, with one tile shape; dw's K dimension (the
-  // rows) is cut so that its work items are about as long as dx's.
+  // Both products run in one launch, with one tile shape, dw's work items first; item
+  // i goes to CTA (pair) i mod slots. dw's K dimension (the rows) is cut into as many
+  // parts as give the shortest of the longest queues, in slices of 64 along K plus one
+  // an item; each part costs the writing and reading of its fp32 sums (about what the
+  // SMs' share of half a slice takes, at 16 floats a thread and tile).
   b.tile = pick_tile(std::max<int64_t>(m, n), k, sms);
+  const int slots = b.tile.slots(sms);
   const int64_t tiles = ceil_div(n, 128 * b.tile.cg) * ceil_div(k, b.tile.bn);
-  const int64_t kblocks = ceil_div(m, 64);
-  const int64_t by_length = ceil_div(kblocks, std::max<int64_t>(4, ceil_div(n, 64)));
-  const int64_t by_slots = std::max<int64_t>(1, 4 * b.tile.slots(sms) / tiles);
+  const int64_t dx_items = ceil_div(m, 128 * b.tile.cg) * ceil_div(k, b.tile.bn);
+  const int64_t dx_len = ceil_div(n, 64) + 1, kblocks = ceil_div(m, 64);
+  int64_t best = 0;
+  b.splits = 1;
+  for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32}) {
+    if (s > kblocks) break;
+    const int64_t kper = ceil_div(kblocks, s), parts = ceil_div(kblocks, kper);
+    const int64_t dw_items = tiles * parts, dw_len = kper + 1;
+    // Queue of slot 0, and of the first slot past dw's last round, which gets one dw item less.
+    const int64_t total = dw_items + dx_items;
+    const auto queue = [&](int64_t slot) {
+      const int64_t dw = slot < dw_items ? (dw_items - slot + slots - 1) / slots : 0;
+      const int64_t all = slot < total ? (total - slot + slots - 1) / slots : 0;
+      return dw * dw_len + (all - dw) * dx_len;
+    };
+    int64_t time = std::max(queue(0), queue(dw_items % slots));
+    if (parts > 1) time += 2 + 3 * parts * tiles / slots;
+    if (best == 0 || time < best) {
+      best = time;
+      b.splits = static_cast<int>(parts);
+    }
+  }
   GemmProblem p{};
-  set_shape(&p, b.tile, n, k, m, static_cast<int>(std::max<int64_t>(1, std::min(by_length, by_slots))));
+  set_shape(&p, b.tile, n, k, m, b.splits);
   b.splits = p.splits;
   b.db_parts = linear_dz_parts(m, n, sms);
   b.dz_stride = (static_cast<int64_t>(n) + 7) / 8 * 8;
@@ -297,24 +328,25 @@ cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_
   if ((st = check_operand(w, w_stride, k, "w")) != CVS_OK) return st;
   if ((st = device_info(&dev)) != CVS_OK) return st;
   const Tile t = pick_tile(m, n, dev.sms);
-  CUtensorMap maps[4];
-  if ((st = operand_map(&maps[0], {x, x_stride, false}, dtype, m, k, 128)) != CVS_OK) return st;
-  if ((st = operand_map(&maps[1], {w, w_stride, false}, dtype, n, k, t.bn / t.cg)) != CVS_OK) return st;
-  maps[2] = maps[0];
-  maps[3] = maps[1];
+  GemmMaps maps{};
+  if ((st = operand_map(&maps.a[0], {x, x_stride, false}, dtype, m, k, 128)) != CVS_OK) return st;
+  if ((st = operand_map(&maps.b[0], {w, w_stride, false}, dtype, n, k, t.bn / t.cg)) != CVS_OK) return st;
   GemmArgs a{};
   GemmProblem& p = a.p[0];
   set_shape(&p, t, m, n, k, 1);
   p.act = activation;
   p.out = y;
   p.ld_out = y_stride;
-  p.vec_out = aligned16(y) && y_stride % 8 == 0;
+  p.vec_out = mappable(y, y_stride, n);
   p.bias = bias;
   p.residual = residual;
   p.ld_res = residual_stride;
-  p.vec_res = aligned16(residual) && residual_stride % 8 == 0;
+  p.vec_res = mappable(residual, residual_stride, n);
   p.z = z;
   p.ld_z = z_stride;
+  if (p.vec_out && (st = block_map(&maps.out[0], y, dtype, m, n, y_stride)) != CVS_OK) return st;
+  if (p.vec_res && (st = block_map(&maps.residual, residual, dtype, m, n, residual_stride)) != CVS_OK) return st;
+  if (z && (st = block_map(&maps.z, z, CVS_F16, m, n, z_stride)) != CVS_OK) return st;
   a.bf16 = dtype == CVS_BF16;
   a.err = dev.err;
   e = gemm_launch(t.cg, t.bn, maps, a, grid_ctas(t, p.work, dev.sms), s);
@@ -383,7 +415,7 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
   }
   const Tile& t = plan.tile;
   if (dx || dw) {
-    CUtensorMap maps[4];
+    GemmMaps maps{};
     GemmArgs a{};
     a.bf16 = bf16;
     a.err = dev.err;
@@ -394,10 +426,11 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
       p.a_mn = p.b_mn = 1;
       p.out = dw;
       p.ld_out = dw_stride;
-      p.vec_out = aligned16(dw) && dw_stride % 8 == 0;
+      p.vec_out = mappable(dw, dw_stride, k);
       p.partial = p.splits > 1 ? reinterpret_cast<float*>(base + plan.dw_offset) : nullptr;
-      if ((st = operand_map(&maps[2 * i], {dz.p, dz.stride, true}, dtype, n, m, 64)) != CVS_OK) return st;
-      if ((st = operand_map(&maps[2 * i + 1], {x, x_stride, true}, dtype, k, m, 64)) != CVS_OK) return st;
+      if ((st = operand_map(&maps.a[i], {dz.p, dz.stride, true}, dtype, n, m, 64)) != CVS_OK) return st;
+      if ((st = operand_map(&maps.b[i], {x, x_stride, true}, dtype, k, m, 64)) != CVS_OK) return st;
+      if (p.vec_out && (st = block_map(&maps.out[i], dw, dtype, n, k, dw_stride)) != CVS_OK) return st;
       ++i;
     }
     if (dx) {  // dx[m][k] = dz w: w has K (its n rows) as its outer dimension
@@ -406,14 +439,11 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
       p.b_mn = 1;
       p.out = dx;
       p.ld_out = dx_stride;
-      p.vec_out = aligned16(dx) && dx_stride % 8 == 0;
-      if ((st = operand_map(&maps[2 * i], dz, dtype, m, n, 128)) != CVS_OK) return st;
-      if ((st = operand_map(&maps[2 * i + 1], {w, w_stride, true}, dtype, k, n, 64)) != CVS_OK) return st;
+      p.vec_out = mappable(dx, dx_stride, k);
+      if ((st = operand_map(&maps.a[i], dz, dtype, m, n, 128)) != CVS_OK) return st;
+      if ((st = operand_map(&maps.b[i], {w, w_stride, true}, dtype, k, n, 64)) != CVS_OK) return st;
+      if (p.vec_out && (st = block_map(&maps.out[i], dx, dtype, m, k, dx_stride)) != CVS_OK) return st;
       ++i;
-    }
-    if (i == 1) {
-      maps[2] = maps[0];
-      maps[3] = maps[1];
     }
     const int work = a.p[0].work + a.p[1].work;
     if ((e = gemm_launch(t.cg, t.bn, maps, a, grid_ctas(t, work, dev.sms), s)) != cudaSuccess)
@@ -432,6 +462,7 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
   f.bn = t.bn;
   f.dw = dw;
   f.ld_dw = dw_stride;
+  f.vec_dw = dw && aligned16(dw) && dw_stride % 8 == 0;
   f.n = n;
   f.k = k;
   f.bf16 = bf16;

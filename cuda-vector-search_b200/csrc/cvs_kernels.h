@@ -244,16 +244,23 @@ struct GemmProblem {
   long long ld_res;
   void* z;               // pre-activation, fp16, rows 16-byte aligned, or null
   long long ld_z;
-  int vec_out, vec_res;  // rows 16-byte aligned
+  int vec_out, vec_res;  // rows the tensor-memory accelerator can address
   float* partial;        // splits > 1: fp32 parts instead of all of the above
 };
+// Only p[0] may have a residual or z.
 struct GemmArgs {
   GemmProblem p[2];
   int bf16;
   int* err;
 };
-// Tile shapes: cg CTAs (128 rows each) x bn columns. maps: A and B of both products.
-cudaError_t gemm_launch(int cg, int bn, const CUtensorMap (&maps)[4], const GemmArgs& a, int ctas, cudaStream_t stream);
+// Tensor maps: both products' operands (boxes as the tile shape needs them) and, in
+// boxes of 64 columns x 32 rows, what the epilogue moves: results (where vec_out),
+// z and the residual (where vec_res).
+struct GemmMaps {
+  CUtensorMap a[2], b[2], out[2], z, residual;
+};
+// Tile shapes: cg CTAs (128 rows each) x bn columns.
+cudaError_t gemm_launch(int cg, int bn, const GemmMaps& maps, const GemmArgs& a, int ctas, cudaStream_t stream);
 
 struct LinearSmallArgs {
   const void* x;
@@ -290,6 +297,7 @@ struct LinearFinishArgs {
   int splits, tiles_m, tiles_n, cg, bn;
   void* dw;
   long long ld_dw;
+  int vec_dw;               // rows 16-byte aligned
   int n, k;                 // dw is [n][k]
   int bf16;
 };
