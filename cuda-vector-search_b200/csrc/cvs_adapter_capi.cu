@@ -540,6 +540,7 @@ cvs_status cvs_preference_loss(const void* q, int q_dtype, int64_t q_stride, con
   a.grad = grad;
   a.grad_stride = grad_stride;
   a.partial = static_cast<float2*>(workspace);
+  a.err = dev.err;
   const cudaError_t e = preference_launch(a, mean, loss, weight, dev.sms, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? CVS_OK : cuda_fail(e, "preference loss launch");
 }

@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 namespace cvs {
 
@@ -21,6 +22,46 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Base-2 exponential and reciprocal of the special-function unit (2 ulp and 1 ulp).
+__device__ __forceinline__ float exp2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Two fp32 values in one register pair, for the instructions that work on both.
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair_of(float lo, float hi) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ void split(Pair p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v));
+}
+__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
+  Pair p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return p;
+}
+__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
+  Pair p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+__device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
+  Pair p;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
 
 // Eight elements as stored: 16 bytes (halves) or 32 bytes (fp32).
 template <class T>
@@ -54,6 +95,41 @@ __device__ __forceinline__ void store8(T* p, const Raw8<T>& r) {
 #pragma unroll
   for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i) d[i] = s[i];
 }
+
+// Elements 2 i and 2 i + 1 of eight, as fp32.
+template <class T>
+__device__ __forceinline__ Pair pair_at(const Raw8<T>& r, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return pair_of(r.v[2 * i], r.v[2 * i + 1]);
+  } else {
+    const uint32_t u = reinterpret_cast<const uint32_t*>(&r)[i];
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return pair_of(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+      return pair_of(f.x, f.y);
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ void set_pair(Raw8<T>& r, int i, Pair p) {
+  float lo, hi;
+  split(p, lo, hi);
+  if constexpr (sizeof(T) == 4) {
+    r.v[2 * i] = lo;
+    r.v[2 * i + 1] = hi;
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    reinterpret_cast<__nv_bfloat162*>(&r)[i] = __floats2bfloat162_rn(lo, hi);
+  } else {
+    reinterpret_cast<__half2*>(&r)[i] = __floats2half2_rn(lo, hi);
+  }
+}
+__device__ __forceinline__ float pair_total(Pair p) {
+  float lo, hi;
+  split(p, lo, hi);
+  return lo + hi;
+}
+__device__ __forceinline__ Pair both(float v) { return pair_of(v, v); }
 
 // The j-th group of eight columns that thread `tid` of `threads` owns in a row
 // of d columns. Aligned rows (VEC): eight consecutive columns, one 16-byte (or

@@ -324,7 +324,9 @@ struct PreferenceArgs {
   float* grad;              // [b][grad_stride] sums of the loss's gradient, or null
   long long grad_stride;    // d rounded up to a multiple of 8
   float2* partial;          // [blocks] (loss, pairs)
-  int warps_per_query;      // set by preference_launch
+  int* err;
+  int warps_per_query;      // set by preference_launch, as is
+  int stage_rows;           // row buffers of each of a warp's two stages
 };
 int preference_blocks(long long b, int r, int num_sms);
 cudaError_t preference_launch(PreferenceArgs a, int mean, float* loss, float* weight, int num_sms, cudaStream_t stream);

@@ -46,48 +46,11 @@ __device__ constexpr float kTail[10] = {-0.9999968409538269f, 1.151208758354187f
                                         -1.8347012797903517e-08f};
 constexpr float kLog2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float exp2_approx(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float rcp_approx(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 // The larger of the two; NaN if either is.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
-}
-
-struct Pair {
-  uint64_t v;
-};
-__device__ __forceinline__ Pair pair_of(float lo, float hi) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
-  return p;
-}
-__device__ __forceinline__ void split(Pair p, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v));
-}
-__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
-  Pair p;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return p;
-}
-__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
-  Pair p;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
-  return p;
-}
-__device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
-  Pair p;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
-  return p;
 }
 
 // Q(-b) of two elements, b = max(-|z|, -7).
@@ -566,7 +529,8 @@ __global__ void __launch_bounds__(GemmShape<CG, BN>::kThreads, 1)
 #pragma unroll
       for (int c = 0; c < kSteps; ++c)
         bias_r[c] = p.bias && col0 + 32 * c + lane < p.n ? half_at(p.bias, col0 + 32 * c + lane, bf16) : 0.f;
-      if (!mbar_wait(sh.tfull(acc), (n >> 1) & 1, abort, args.err, 36)) break;
+      // One answer for the warp: what follows is done by all its lanes or by none.
+      if (!__all_sync(0xffffffffu, mbar_wait(sh.tfull(acc), (n >> 1) & 1, abort, args.err, 36))) break;
       tc_fence_after();
       // The accumulator is free once its last 32 columns are in registers.
       const auto release = [&]() {
@@ -653,7 +617,7 @@ __global__ void __launch_bounds__(GemmShape<CG, BN>::kThreads, 1)
         act_values(v, act);
         if (residual) {
           if (p.vec_res && (c & 1) == 0) {
-            ok = mbar_wait(sh.rfull(ew, b), (rphase >> b) & 1, abort, args.err, 37) && ok;
+            ok = __all_sync(0xffffffffu, mbar_wait(sh.rfull(ew, b), (rphase >> b) & 1, abort, args.err, 37)) && ok;
             rphase ^= 1u << b;
           }
           buf_add(buf, lane, c & 1, v, bf16);

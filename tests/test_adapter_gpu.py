@@ -329,8 +329,11 @@ def check_preference(cvs, index, q, chosen, rejected, ref=None, scale=5.0, smoot
     cosine = index.metric == "cosine"
     x = index.embeddings
     want_loss, want_m, want_dq = oracle.preference(q.detach(), ref, chosen, rej, x, cosine, scale, smoothing, reduction == "mean")
-    # Margins: products of d components, each of u and u_ref off by 60 e of itself
-    # (norm, division, difference), summed with 80 e of their magnitudes.
+    # Margins: scale (u.x_c - u.x_r), each of u and u_ref off by 60 e of itself (norm,
+    # division, difference), each sum of d products off by 80 e of its magnitudes, which
+    # are |u| (|x_c| + |x_r|) together.
+    # Gradient: fl(S x_c - sum_j s_j x_j), S = fl(sum_j s_j) of r slopes: at most r + 2
+    # roundings of partial sums no larger than sum_j |s_j| (|x_c| + |x_j|); r <= 64.
     qd = q.detach().double()
     mag = qd / qd.norm(dim=1, keepdim=True).clamp_min(1e-12) if cosine else qd
     mag = mag.abs()
@@ -338,8 +341,9 @@ def check_preference(cvs, index, q, chosen, rejected, ref=None, scale=5.0, smoot
         rd = ref.double()
         mag = mag + (rd / rd.norm(dim=1, keepdim=True).clamp_min(1e-12) if cosine else rd).abs()
     there = (chosen[:, None] >= 0) & (rej >= 0)
-    apart = (x.double()[chosen.clamp_min(0)][:, None] - x.double()[rej.clamp_min(0)]).abs()
-    m_err = torch.where(there, scale * 150 * E * (apart * mag[:, None]).sum(2), 0.0)
+    xc, xr = x.double()[chosen.clamp_min(0)][:, None], x.double()[rej.clamp_min(0)]
+    apart, sizes = (xc - xr).abs(), xc.abs() + xr.abs()
+    m_err = torch.where(there, scale * 150 * E * (sizes * mag[:, None]).sum(2), 0.0)
     oracle.close(margins, want_m, m_err + 4 * E * want_m.abs())
     pairs = max(int(there.sum()), 1)
     weight = 1.0 / pairs if reduction == "mean" else 1.0
@@ -347,7 +351,7 @@ def check_preference(cvs, index, q, chosen, rejected, ref=None, scale=5.0, smoot
     # Gradient: slopes change by at most a quarter per unit of m.
     slope_err = torch.where(there, 0.25 * m_err + 16 * E, 0.0) * scale * weight
     slope = torch.where(there, torch.ones_like(m_err), 0.0) * scale * weight
-    du_err = (slope_err[:, :, None] * apart).sum(1) + 100 * E * (slope[:, :, None] * apart).sum(1)
+    du_err = (slope_err[:, :, None] * apart).sum(1) + 100 * E * (slope[:, :, None] * sizes).sum(1)
     if cosine:
         n = qd.norm(dim=1, keepdim=True).clamp_min(1e-12)
         u = (qd / n).abs()
