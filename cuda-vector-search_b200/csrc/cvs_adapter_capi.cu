@@ -281,6 +281,7 @@ cvs_status cvs_layer_norm_backward(const void* dy, int64_t dy_stride, const void
   a.dweight = dweight;
   a.dbias = dbias;
   a.partial = sums ? static_cast<float*>(workspace) : nullptr;
+  a.err = dev.err;
   const cudaError_t e = norm_launch(a, dtype, true, dev.sms, s);
   return e == cudaSuccess ? CVS_OK : cuda_fail(e, "layer norm backward launch");
 }

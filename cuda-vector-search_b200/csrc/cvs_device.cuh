@@ -166,6 +166,15 @@ __device__ __forceinline__ void tma_load_2d_to_pair_bar(void* smem_dst, const vo
       : "memory");
 }
 
+// Copies `bytes` (a multiple of 16, both addresses 16-byte aligned) to shared memory,
+// completion on an mbarrier that expects them.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // tcgen05: tensor memory, MMA, commit, loads
 // ---------------------------------------------------------------------------

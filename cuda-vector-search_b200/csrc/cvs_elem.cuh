@@ -77,6 +77,15 @@ __device__ __forceinline__ Raw8<T> zero8() {
   return r;
 }
 
+// Hides the elements' history from the compiler, which would otherwise keep their
+// converted values in registers from one use to the next instead of converting again.
+template <class T>
+__device__ __forceinline__ void forget(Raw8<T>& r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(r) / 4); ++i) asm volatile("" : "+r"(u[i]));
+}
+
 // p must be 16-byte aligned.
 template <class T>
 __device__ __forceinline__ Raw8<T> load8(const T* p) {

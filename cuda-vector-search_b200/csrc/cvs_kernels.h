@@ -218,6 +218,8 @@ struct NormArgs {
   void* dweight;       // null: not wanted
   void* dbias;
   float* partial;      // [blocks][2][d] or null when neither dweight nor dbias is wanted
+  int* err;
+  int slots;           // set by norm_launch: row pairs in a warp's ring
 };
 // Blocks of the backward kernel, each with its own row of `partial`.
 int norm_backward_blocks(long long rows, int d, int num_sms);

@@ -33,31 +33,37 @@ namespace {
 // Activations
 // ---------------------------------------------------------------------------
 // GELU z Phi(z) = max(z, 0) - |z| Q(|z|) with the tail probability Q(a) = Phi(-a) as
-// 2^P(-a): log2 Q is smooth and nearly quadratic, so a degree-9 polynomial (a
-// least-squares fit on 0 .. 7 reweighted towards the smallest largest error) gives Q
-// to 6e-6 relative everywhere, tails included, for nine multiply-adds and one ex2.
-// Beyond 7, where |z| Q < 1e-11, Q(7) stands in. The multiply-adds run on pairs
-// (fma.rn.f32x2), two elements an instruction. With erff the epilogue, not the tensor
-// cores, set the pace: 16384 x 768 -> 1536 took 112 us, against 47 us without an
-// activation.
-__device__ constexpr float kTail[10] = {-0.9999968409538269f, 1.151208758354187f,      -0.4586543142795563f,
-                                        0.053635455667972565f, 0.008232222869992256f,  0.0007997678476385772f,
-                                        2.531037353037391e-05f, -4.018034360342426e-06f, -5.080352138975286e-07f,
-                                        -1.8347012797903517e-08f};
+// 2^P(-a): log2 Q is smooth and nearly quadratic, so a degree-7 polynomial (a
+// least-squares fit on 0 .. 6 reweighted towards the smallest largest error) gives Q
+// to 6e-6 relative everywhere, tails included, for seven multiply-adds and one ex2.
+// Beyond 6, where |z| Q(|z|) < 6e-9 (fp16 rounds it to zero), Q(6) stands in. The
+// multiply-adds run on pairs (fma.rn.f32x2), two elements an instruction. With erff the
+// epilogue, not the tensor cores, set the pace: 16384 x 768 -> 1536 took 112 us, against
+// 47 us without an activation.
+constexpr float kTailEnd = 6.f;
+__device__ constexpr float kTail[8] = {-0.9999952912330627f, 1.1512510776519775f,     -0.4584643840789795f,
+                                       0.05396007001399994f, 0.00850789062678814f,   0.0009305247804149985f,
+                                       6.159828626550734e-05f, 1.8348112007515738e-06f};
 constexpr float kLog2E = 1.4426950408889634f;
 
-// The larger of the two; NaN if either is.
+// The larger (smaller) of the two; NaN if either is.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
-// Q(-b) of two elements, b = max(-|z|, -7).
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Q(-b) of two elements, b = max(-|z|, -kTailEnd).
 __device__ __forceinline__ void tail_pair(Pair b, float& q0, float& q1) {
-  Pair p = pair_of(kTail[9], kTail[9]);
+  Pair p = both(kTail[7]);
 #pragma unroll
-  for (int i = 8; i >= 0; --i) p = pair_fma(p, b, pair_of(kTail[i], kTail[i]));
+  for (int i = 6; i >= 0; --i) p = pair_fma(p, b, both(kTail[i]));
   float p0, p1;
   split(p, p0, p1);
   q0 = exp2_approx(p0);
@@ -70,7 +76,7 @@ __device__ __forceinline__ void act_pair(float& z0, float& z1) {
     z0 = max_nan(z0, 0.f);
     z1 = max_nan(z1, 0.f);
   } else if constexpr (ACT == kActGelu) {
-    const Pair b = pair_of(fmaxf(-fabsf(z0), -7.f), fmaxf(-fabsf(z1), -7.f));
+    const Pair b = pair_of(fmaxf(-fabsf(z0), -kTailEnd), fmaxf(-fabsf(z1), -kTailEnd));
     float q0, q1;
     tail_pair(b, q0, q1);
     split(pair_fma(b, pair_of(q0, q1), pair_of(max_nan(z0, 0.f), max_nan(z1, 0.f))), z0, z1);
@@ -95,30 +101,34 @@ __device__ __forceinline__ void act_values(float (&v)[N], int act) {
   else if (act == kActSilu) act_values<kActSilu>(v);
 }
 
-// g act'(z) for two elements. z beyond +-100 gives slopes 0 and 1 to the last bit;
-// the clamp keeps an infinite z (an overflowed fp16 pre-activation) from giving
-// inf x 0. NaN stays.
+// g act'(z) for two elements. Beyond +-30 the slopes are 0 and 1 to the last bit; the
+// clamp keeps an infinite z (an overflowed fp16 pre-activation) from giving inf x 0 and
+// passes NaN on.
 template <int ACT>
 __device__ __forceinline__ void slope_pair(float z0, float z1, float& g0, float& g1) {
   if constexpr (ACT == kActRelu) {
     g0 = z0 > 0.f ? g0 : (z0 != z0 ? z0 : 0.f);
     g1 = z1 > 0.f ? g1 : (z1 != z1 ? z1 : 0.f);
-  } else if constexpr (ACT == kActGelu) {
+    return;
+  }
+  const float c0 = min_nan(max_nan(z0, -30.f), 30.f), c1 = min_nan(max_nan(z1, -30.f), 30.f);
+  if constexpr (ACT == kActGelu) {
     // Phi(z) + z phi(z), phi(z) = 2^(-z^2 log2(e) / 2) / sqrt(2 pi).
-    const float c0 = z0 != z0 ? z0 : fminf(fmaxf(z0, -100.f), 100.f), c1 = z1 != z1 ? z1 : fminf(fmaxf(z1, -100.f), 100.f);
     float q0, q1, e0, e1;
-    tail_pair(pair_of(fmaxf(-fabsf(c0), -7.f), fmaxf(-fabsf(c1), -7.f)), q0, q1);
+    tail_pair(pair_of(fmaxf(-fabsf(c0), -kTailEnd), fmaxf(-fabsf(c1), -kTailEnd)), q0, q1);
     const Pair c = pair_of(c0, c1);
-    split(pair_mul(pair_mul(c, c), pair_of(-0.5f * kLog2E, -0.5f * kLog2E)), e0, e1);
+    split(pair_mul(pair_mul(c, both(-0.5f * kLog2E)), c), e0, e1);
     const Pair phi = pair_of(exp2_approx(e0), exp2_approx(e1));
     const Pair cdf = pair_of(c0 > 0.f ? 1.f - q0 : q0, c1 > 0.f ? 1.f - q1 : q1);
-    const Pair s = pair_fma(pair_mul(c, pair_of(0.39894228040143268f, 0.39894228040143268f)), phi, cdf);
+    const Pair s = pair_fma(pair_mul(c, both(0.39894228040143268f)), phi, cdf);
     split(pair_mul(s, pair_of(g0, g1)), g0, g1);
   } else {
-    const float c0 = z0 != z0 ? z0 : fminf(fmaxf(z0, -100.f), 100.f), c1 = z1 != z1 ? z1 : fminf(fmaxf(z1, -100.f), 100.f);
-    const float s0 = rcp_approx(1.f + exp2_approx(-kLog2E * c0)), s1 = rcp_approx(1.f + exp2_approx(-kLog2E * c1));
-    g0 *= s0 * fmaf(c0, 1.f - s0, 1.f);
-    g1 *= s1 * fmaf(c1, 1.f - s1, 1.f);
+    float e0, e1;
+    split(pair_mul(pair_of(c0, c1), both(-kLog2E)), e0, e1);
+    const Pair s = pair_of(rcp_approx(1.f + exp2_approx(e0)), rcp_approx(1.f + exp2_approx(e1)));
+    // s (1 + z (1 - s))
+    const Pair t = pair_fma(pair_of(c0, c1), pair_fma(s, both(-1.f), both(1.f)), both(1.f));
+    split(pair_mul(pair_mul(s, t), pair_of(g0, g1)), g0, g1);
   }
 }
 
@@ -272,22 +282,51 @@ __device__ __forceinline__ void buf_add(const uint8_t* buf, int lane, int h, flo
 // warp's two-byte accesses are consecutive.
 __device__ __forceinline__ void buf_to_rows(const uint8_t* buf, void* dst, long long ld, int row0, int rows, int col0,
                                             int cols, int lane) {
-  for (int r = 0; r < 32 && row0 + r < rows; ++r) {
-    uint16_t* p = static_cast<uint16_t*>(dst) + (row0 + r) * ld + col0;
 #pragma unroll
-    for (int c = lane; c < 64; c += 32)
-      if (col0 + c < cols) p[c] = *reinterpret_cast<const uint16_t*>(buf + buf_at(r, c >> 3) + 2 * (c & 7));
+  for (int r0 = 0; r0 < 32; r0 += 16) {
+    uint16_t v[16][2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = lane + 32 * h;
+        v[r][h] = *reinterpret_cast<const uint16_t*>(buf + buf_at(r0 + r, c >> 3) + 2 * (c & 7));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      uint16_t* p = static_cast<uint16_t*>(dst) + (row0 + r0 + r) * ld + col0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = lane + 32 * h;
+        if (row0 + r0 + r < rows && col0 + c < cols) p[c] = v[r][h];
+      }
+    }
   }
 }
 __device__ __forceinline__ void rows_to_buf(uint8_t* buf, const void* src, long long ld, int row0, int rows, int col0,
                                             int cols, int lane) {
-#pragma unroll 8
-  for (int r = 0; r < 32; ++r) {
-    const uint16_t* p = static_cast<const uint16_t*>(src) + (row0 + r) * ld + col0;
+  // Sixteen rows' loads are under way before the first of them is staged.
 #pragma unroll
-    for (int c = lane; c < 64; c += 32)
-      *reinterpret_cast<uint16_t*>(buf + buf_at(r, c >> 3) + 2 * (c & 7)) =
-          row0 + r < rows && col0 + c < cols ? p[c] : static_cast<uint16_t>(0);
+  for (int r0 = 0; r0 < 32; r0 += 16) {
+    uint16_t v[16][2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const uint16_t* p = static_cast<const uint16_t*>(src) + (row0 + r0 + r) * ld + col0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = lane + 32 * h;
+        v[r][h] = row0 + r0 + r < rows && col0 + c < cols ? p[c] : static_cast<uint16_t>(0);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = lane + 32 * h;
+        *reinterpret_cast<uint16_t*>(buf + buf_at(r0 + r, c >> 3) + 2 * (c & 7)) = v[r][h];
+      }
+    }
   }
 }
 
@@ -567,21 +606,17 @@ __global__ void __launch_bounds__(GemmShape<CG, BN>::kThreads, 1)
         const int b = keeps_z ? 0 : (n * kChunks + (c >> 1)) & 1;
         uint8_t* buf = bufs + b * kBufBytes;
         const bool live = row0 < p.m && cc < p.n;
-        if ((c & 1) == 0) {
-          // A new block: its buffer's last one has left. A residual's block comes one
-          // ahead into the other buffer.
+        if ((c & 1) == 0 && residual) {
+          // The residual's block comes into the buffer that its result will leave from,
+          // one block ahead into the other buffer where that is free.
           if (lane == 0) {
-            if (keeps_z || ahead) tma_store_wait_read<0>();
-            else tma_store_wait_read<1>();
-            if (ahead) {
-              if (c + 2 < kSteps) request(t, (c >> 1) + 1, b ^ 1);
-              else request(t + step, 0, b ^ 1);
-            } else {
-              request(t, c >> 1, b);
-            }
+            tma_store_wait_read<0>();
+            if (!ahead) request(t, c >> 1, b);
+            else if (c + 2 < kSteps) request(t, (c >> 1) + 1, b ^ 1);
+            else request(t + step, 0, b ^ 1);
           }
           __syncwarp();
-          if (live && residual && !p.vec_res) {
+          if (live && !p.vec_res) {
             rows_to_buf(buf, p.residual, p.ld_res, row0, p.m, cc, p.n, lane);
             __syncwarp();
           }
@@ -602,6 +637,14 @@ __global__ void __launch_bounds__(GemmShape<CG, BN>::kThreads, 1)
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(now[i]);
+        }
+        if ((c & 1) == 0 && !residual) {
+          // A new block's first values: its buffers' last blocks have left.
+          if (lane == 0) {
+            if (z) tma_store_wait_read<0>();
+            else tma_store_wait_read<1>();
+          }
+          __syncwarp();
         }
         if (z) {
           if (act == kActRelu) {
@@ -926,7 +969,7 @@ cudaError_t linear_small_launch(const LinearSmallArgs& a, cudaStream_t stream) {
 
 int linear_dz_parts(long long m, int n, int num_sms) {
   const int cols = (n + kDzCols - 1) / kDzCols;
-  const long long want = std::max(1, 8 * num_sms / cols);
+  const long long want = std::max(1, 2 * num_sms / cols);  // one round of blocks, few sums to add
   return static_cast<int>(std::max<long long>(1, std::min<long long>(want, (m + kDzWarps - 1) / kDzWarps)));
 }
 

@@ -12,18 +12,19 @@
 // rows far from zero lose nothing. All sums are fp32.
 //
 // A row belongs to one warp (width up to 1024: no barrier) or to one block of 8 warps
-// (up to 8192). Weights are held as fp32 pairs in shared memory, in the order the lanes
-// read them. Forward, a warp takes two rows at a time, which doubles the loads in flight
-// and halves the reads of the weights. In the backward pass a block walks rows with a
-// stride of the grid, the next row's loads under way, and every thread keeps the sums of
-// dw and db for the columns it owns, so the weights' gradients cost no traffic per row;
-// the blocks' sums go to the workspace and a second small kernel adds them in a fixed
-// order, which makes the result the same on every run.
+// (up to 8192). Aligned rows of one warp come as bulk copies into a ring per warp in
+// shared memory (forward: from 16384 rows on), so that the bytes in flight cost no
+// registers and each SM's warps never wait for one another's rows. In the backward pass
+// every thread keeps the sums of dw and db for the columns it owns while its warp walks
+// the rows, so the weights' gradients cost no traffic per row; the blocks' sums go to the
+// workspace and a second small kernel adds them in a fixed order, which makes the result
+// the same on every run.
 #include "cvs_device.cuh"
 #include "cvs_elem.cuh"
 #include "cvs_kernels.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace cvs {
 
@@ -31,6 +32,8 @@ namespace {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormWarps = kNormThreads / 32;
+constexpr int kNormSlots = 4;    // most row pairs in a warp's ring of the backward pass
+constexpr int kForwardSlots = 8; // most rows in a warp's ring of the forward pass
 constexpr int kForwardRows = 2;  // rows a warp has at work in the forward pass
 
 // Sum over the threads of a row: one warp, or all 8 warps of the block (scratch
@@ -53,23 +56,38 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* scratch) {
   return make_float2(a, b);
 }
 
-// Weights of the thread's columns as fp32 pairs: group j, pair i at [(j * 4 + i) * threads
-// + tid], one conflict-free 8-byte read.
+// Weights of a row's threads as fp32 pairs: group j, pair i of thread tid at [(j * 4 + i)
+// * THREADS + tid], one conflict-free 8-byte read. Staged by the whole block.
 template <class T, bool VEC, int THREADS, int CPL>
-__device__ __forceinline__ void stage_weights(const void* w, bool w32, int d, int tid, float missing, float2* out) {
+__device__ __forceinline__ void stage_weights(const void* w, bool w32, int d, float2* out) {
 #pragma unroll
-  for (int j = 0; j < CPL; ++j) {
+  for (int k = threadIdx.x; k < CPL * 4 * THREADS; k += kNormThreads) {
+    const int tid = k % THREADS, i = k / THREADS % 4, j = k / THREADS / 4;
+    float v[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float v[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int c = Cols<VEC>::at(tid, THREADS, j, 2 * i + t);
-        v[t] = missing;
-        if (w != nullptr && c < d) v[t] = w32 ? static_cast<const float*>(w)[c] : to_f32(static_cast<const T*>(w)[c]);
-      }
-      out[(j * 4 + i) * THREADS + tid] = make_float2(v[0], v[1]);
+    for (int t = 0; t < 2; ++t) {
+      const int c = Cols<VEC>::at(tid, THREADS, j, 2 * i + t);
+      v[t] = 0.f;
+      if (c < d) v[t] = w32 ? static_cast<const float*>(w)[c] : to_f32(static_cast<const T*>(w)[c]);
     }
+    out[k] = make_float2(v[0], v[1]);
+  }
+}
+// Group j of the thread's weights straight from global memory (L1).
+template <class T, bool VEC>
+__device__ __forceinline__ void weight_group(const void* w, bool w32, int d, int tid, int threads, int j, float missing,
+                                             Pair (&out)[4]) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = both(missing);
+  } else if (w32) {
+    const Raw8<float> r = Cols<VEC>::load(static_cast<const float*>(w), d, tid, threads, j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = pair_at(r, i);
+  } else {
+    const Raw8<T> r = Cols<VEC>::load(static_cast<const T*>(w), d, tid, threads, j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = pair_at(r, i);
   }
 }
 template <int THREADS>
@@ -88,33 +106,71 @@ __device__ __forceinline__ Pair inside(Pair p, int d, int tid, int threads, int 
   return pair_of(lo, hi);
 }
 
-template <class T, bool VEC, int WARPS, int CPL>
-__global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const NormArgs a) {
+template <bool VEC, int WARPS>
+__host__ __device__ constexpr bool norm_ring() { return VEC && WARPS == 1; }
+
+// STAGED: weights in shared memory, for blocks that walk many rows; otherwise straight
+// from global memory, where the staging and its barrier would be a large part of the
+// work (256 rows of 768: 5.2 us staged, 4.3 us straight; 262144 rows: 137 and 185 us).
+template <class T, bool VEC, int WARPS, int CPL, bool STAGED>
+__global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int kRowThreads = 32 * WARPS;
   constexpr int kRowsPerBlock = kNormThreads / kRowThreads;
-  constexpr int kRows = WARPS == 1 ? kForwardRows : 1;  // rows a warp (block) has at work
+  constexpr bool kRing = STAGED && norm_ring<VEC, WARPS>();
+  constexpr int kRows = WARPS == 1 && !kRing ? kForwardRows : 1;  // rows a warp (block) has at work
   __shared__ float2 scratch[2][WARPS > 1 ? WARPS : 1];
-  extern __shared__ float2 weights[];  // [2][CPL * 4][kRowThreads]
+  __shared__ __align__(8) uint64_t bars[kRing ? kNormWarps : 1][kRing ? kForwardSlots : 1];
+  __shared__ int abort_s;
+  extern __shared__ __align__(128) uint8_t shared_f[];  // STAGED: weight and bias, [2][CPL * 4][kRowThreads]; the ring
+  const float2* weight_s = reinterpret_cast<const float2*>(shared_f);
+  const float2* bias_s = weight_s + CPL * 4 * kRowThreads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tid = threadIdx.x % kRowThreads;
   const int d = a.d;
   const float inv_d = 1.f / static_cast<float>(d);
-  float2* w_s = weights;
-  float2* b_s = weights + CPL * 4 * kRowThreads;
-  grid_dependency_wait();
-  if (threadIdx.x < kRowThreads) {
-    if (a.weight) stage_weights<T, VEC, kRowThreads, CPL>(a.weight, a.w32, d, tid, 1.f, w_s);
-    if (a.bias) stage_weights<T, VEC, kRowThreads, CPL>(a.bias, a.w32, d, tid, 0.f, b_s);
+  if constexpr (kRing) {
+    if (lane == 0) {
+      for (int k = 0; k < a.slots; ++k) mbar_init(&bars[warp][k], 1);
+      if (warp == 0) abort_s = 0;
+      fence_barrier_init();
+    }
   }
-  __syncthreads();
+  grid_dependency_wait();
+  if constexpr (STAGED) {
+    float2* out = reinterpret_cast<float2*>(shared_f);
+    if (a.weight) stage_weights<T, VEC, kRowThreads, CPL>(a.weight, a.w32, d, out);
+    if (a.bias) stage_weights<T, VEC, kRowThreads, CPL>(a.bias, a.w32, d, out + CPL * 4 * kRowThreads);
+    __syncthreads();
+  }
   const long long slots = static_cast<long long>(gridDim.x) * kRowsPerBlock;
-  for (long long row0 = static_cast<long long>(blockIdx.x) * kRowsPerBlock + threadIdx.x / kRowThreads; row0 < a.rows;
-       row0 += slots * kRows) {
+  long long row0 = static_cast<long long>(blockIdx.x) * kRowsPerBlock + threadIdx.x / kRowThreads;
+  const uint32_t row_bytes = static_cast<uint32_t>(d) * sizeof(T);
+  uint8_t* ring = shared_f + 2 * CPL * 4 * kRowThreads * sizeof(float2) + static_cast<size_t>(warp) * a.slots * row_bytes;
+  const auto request = [&](long long r, int k) {  // one lane
+    if (r >= a.rows) return;
+    mbar_arrive_expect_tx(&bars[warp][k], row_bytes);
+    bulk_load(ring + k * row_bytes, static_cast<const T*>(a.x) + r * a.x_stride, row_bytes, &bars[warp][k]);
+  };
+  if constexpr (kRing) {
+    if (lane == 0) {
+      for (int k = 0; k < a.slots; ++k) request(row0 + k * slots, k);
+    }
+  }
+  int slot = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  for (; row0 < a.rows; row0 += slots * kRows) {
     Raw8<T> raw[kRows][CPL];
     float mean[kRows], rstd[kRows];
+    if constexpr (kRing) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][slot], parity, &abort_s, a.err, 42));
+      if (!ok) break;
+    }
 #pragma unroll
     for (int q = 0; q < kRows; ++q) {
       const long long row = row0 + q * slots;
-      const T* x = static_cast<const T*>(a.x) + (row < a.rows ? row : row0) * a.x_stride;
+      const T* x = kRing ? reinterpret_cast<const T*>(ring + slot * row_bytes)
+                         : static_cast<const T*>(a.x) + (row < a.rows ? row : row0) * a.x_stride;
 #pragma unroll
       for (int j = 0; j < CPL; ++j) raw[q][j] = Cols<VEC>::load(x, d, tid, kRowThreads, j);
     }
@@ -127,6 +183,14 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const NormAr
         for (int i = 0; i < 4; ++i) sum = pair_add(sum, pair_at(raw[q][j], i));
       }
       mean[q] = row_sum2<WARPS>(pair_total(sum), 0.f, scratch[0]).x * inv_d;
+    }
+    if constexpr (kRing) {
+      // Every lane has its part of the row in registers (the sum needed all of them).
+      if (lane == 0) request(row0 + a.slots * slots, slot);
+      if (++slot == a.slots) {
+        slot = 0;
+        parity ^= 1;
+      }
     }
 #pragma unroll
     for (int q = 0; q < kRows; ++q) {
@@ -154,14 +218,23 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const NormAr
 #pragma unroll
     for (int j = 0; j < CPL; ++j) {
       Raw8<T> out[kRows];
+      Pair w[4], b[4];
+      if constexpr (STAGED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = a.weight ? weight_at<kRowThreads>(weight_s, tid, j, i) : both(1.f);
+          b[i] = a.bias ? weight_at<kRowThreads>(bias_s, tid, j, i) : both(0.f);
+        }
+      } else {
+        weight_group<T, VEC>(a.weight, a.w32, d, tid, kRowThreads, j, 1.f, w);
+        weight_group<T, VEC>(a.bias, a.w32, d, tid, kRowThreads, j, 0.f, b);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const Pair w = a.weight ? weight_at<kRowThreads>(w_s, tid, j, i) : both(1.f);
-        const Pair b = a.bias ? weight_at<kRowThreads>(b_s, tid, j, i) : both(0.f);
 #pragma unroll
         for (int q = 0; q < kRows; ++q) {
           const Pair h = pair_mul(pair_add(pair_at(raw[q][j], i), both(-mean[q])), both(rstd[q]));
-          set_pair(out[q], i, pair_fma(h, w, b));
+          set_pair(out[q], i, pair_fma(h, w[i], b[i]));
         }
       }
 #pragma unroll
@@ -171,17 +244,33 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const NormAr
       }
     }
   }
+  if constexpr (kRing) {
+    if (!ok && lane == 0) {  // after a wait that ran out: copies under way land
+      for (int k = 0; k < a.slots; ++k, row0 += slots) {
+        if (row0 < a.rows) mbar_wait_drain(&bars[warp][(slot + k) % a.slots], slot + k < a.slots ? parity : parity ^ 1);
+      }
+    }
+  }
 }
 
+// Backward. Aligned rows of one warp (kRing) come as bulk copies into a ring of `slots`
+// row pairs (x, dy) per warp in shared memory, so that the bytes in flight cost no
+// registers, which the sums of dw and db need (16 a group of columns); other rows are
+// loaded into registers, the next row's loads under way where that fits. Two blocks an
+// SM, except for wide fp32 rows.
 template <class T, bool VEC, int WARPS, int CPL>
-__global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads, sizeof(T) == 4 && CPL > 3 ? 1 : 2)
+    norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int kRowThreads = 32 * WARPS;
   constexpr int kRowsPerBlock = kNormThreads / kRowThreads;
-  // The next row is fetched while this one is computed where registers allow it.
-  constexpr bool kAhead = sizeof(T) * CPL <= 8;
+  constexpr bool kRing = norm_ring<VEC, WARPS>();
   __shared__ float2 scratch[2][WARPS > 1 ? WARPS : 1];
-  // The weights, and after the last row (single-warp rows) the warps' sums [8][2][d].
-  extern __shared__ float2 shared[];
+  __shared__ __align__(8) uint64_t bars[kRing ? kNormWarps : 1][kRing ? kNormSlots : 1];
+  __shared__ int abort_s;
+  // The weights, then the ring; after the last row (single-warp rows) the warps' sums [8][2][d].
+  extern __shared__ __align__(128) uint8_t shared_b[];
+  float2* shared = reinterpret_cast<float2*>(shared_b);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tid = threadIdx.x % kRowThreads;
   const int d = a.d;
   const float inv_d = 1.f / static_cast<float>(d);
@@ -191,40 +280,60 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormA
 #pragma unroll
     for (int i = 0; i < 4; ++i) dw[j][i] = db[j][i] = both(0.f);
   }
+  if constexpr (kRing) {
+    if (lane == 0) {
+      for (int k = 0; k < a.slots; ++k) mbar_init(&bars[warp][k], 1);
+      if (warp == 0) abort_s = 0;
+      fence_barrier_init();
+    }
+  }
   grid_dependency_wait();
-  if (a.weight && threadIdx.x < kRowThreads)
-    stage_weights<T, VEC, kRowThreads, CPL>(a.weight, a.w32, d, tid, 1.f, shared);
+  if (a.weight) stage_weights<T, VEC, kRowThreads, CPL>(a.weight, a.w32, d, shared);
   __syncthreads();
   const long long slots = static_cast<long long>(gridDim.x) * kRowsPerBlock;
-  Raw8<T> xr[CPL], gr[CPL], xn[CPL], gn[CPL];
-  float mean = 0.f, rstd = 0.f, mean_n = 0.f, rstd_n = 0.f;
-  const auto fetch = [&](long long row, Raw8<T> (&x8)[CPL], Raw8<T> (&g8)[CPL], float& m, float& r) {
-    if (row >= a.rows) return;
-    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
-    m = a.mean[row];
-    r = a.rstd[row];
-#pragma unroll
-    for (int j = 0; j < CPL; ++j) {
-      x8[j] = Cols<VEC>::load(x, d, tid, kRowThreads, j);
-      g8[j] = Cols<VEC>::load(dy, d, tid, kRowThreads, j);
-    }
-  };
-  int turn = 0;
   long long row = static_cast<long long>(blockIdx.x) * kRowsPerBlock + threadIdx.x / kRowThreads;
-  if (kAhead) fetch(row, xn, gn, mean_n, rstd_n);
+  const uint32_t row_bytes = static_cast<uint32_t>(d) * sizeof(T);
+  uint8_t* ring = shared_b + CPL * 4 * kRowThreads * sizeof(float2) + static_cast<size_t>(warp) * a.slots * 2 * row_bytes;
+  const auto request = [&](long long r, int k) {  // one lane
+    if (r >= a.rows) return;
+    mbar_arrive_expect_tx(&bars[warp][k], 2 * row_bytes);
+    bulk_load(ring + k * 2 * row_bytes, static_cast<const T*>(a.x) + r * a.x_stride, row_bytes, &bars[warp][k]);
+    bulk_load(ring + k * 2 * row_bytes + row_bytes, static_cast<const T*>(a.dy) + r * a.dy_stride, row_bytes, &bars[warp][k]);
+  };
+  Raw8<T> xr[CPL], gr[CPL];
+  float mean_n = 0.f, rstd_n = 0.f;
+  if (row < a.rows) {
+    mean_n = a.mean[row];
+    rstd_n = a.rstd[row];
+  }
+  if constexpr (kRing) {
+    if (lane == 0) {
+      for (int k = 0; k < a.slots; ++k) request(row + k * slots, k);
+    }
+  }
+  int turn = 0, slot = 0;
+  uint32_t parity = 0;
+  bool ok = true;
   for (; row < a.rows; row += slots, turn ^= 1) {
-    if constexpr (kAhead) {
+    const float mean = mean_n, rstd = rstd_n;
+    if (row + slots < a.rows) {
+      mean_n = a.mean[row + slots];
+      rstd_n = a.rstd[row + slots];
+    }
+    const T *xs, *gs;  // this row
+    if constexpr (kRing) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][slot], parity, &abort_s, a.err, 41));
+      if (!ok) break;
+      xs = reinterpret_cast<const T*>(ring + slot * 2 * row_bytes);
+      gs = reinterpret_cast<const T*>(ring + slot * 2 * row_bytes + row_bytes);
+    } else {
+      xs = static_cast<const T*>(a.x) + row * a.x_stride;
+      gs = static_cast<const T*>(a.dy) + row * a.dy_stride;
 #pragma unroll
       for (int j = 0; j < CPL; ++j) {
-        xr[j] = xn[j];
-        gr[j] = gn[j];
+        xr[j] = Cols<VEC>::load(xs, d, tid, kRowThreads, j);
+        gr[j] = Cols<VEC>::load(gs, d, tid, kRowThreads, j);
       }
-      mean = mean_n;
-      rstd = rstd_n;
-      fetch(row + slots, xn, gn, mean_n, rstd_n);
-    } else {
-      fetch(row, xr, gr, mean, rstd);
     }
     // h = x r - mu r. Columns outside the row: dy reads as zero there, so g is zero
     // and they add nothing to any sum.
@@ -232,6 +341,10 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormA
     Pair s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
     for (int j = 0; j < CPL; ++j) {
+      if constexpr (kRing) {
+        xr[j] = Cols<VEC>::load(xs, d, tid, kRowThreads, j);
+        gr[j] = Cols<VEC>::load(gs, d, tid, kRowThreads, j);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const Pair g = pair_at(gr[j], i);
@@ -249,6 +362,10 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormA
       T* dx = static_cast<T*>(a.dx) + row * a.dx_stride;
 #pragma unroll
       for (int j = 0; j < CPL; ++j) {
+        if constexpr (sizeof(T) == 2) {
+          forget(xr[j]);
+          forget(gr[j]);
+        }
         Raw8<T> out;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -260,12 +377,28 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormA
         Cols<VEC>::store(dx, d, tid, kRowThreads, j, out);
       }
     }
+    if constexpr (kRing) {
+      __syncwarp();  // the row has been read
+      if (lane == 0) request(row + a.slots * slots, slot);
+      if (++slot == a.slots) {
+        slot = 0;
+        parity ^= 1;
+      }
+    }
+  }
+  if constexpr (kRing) {
+    if (!ok && lane == 0) {  // after a wait that ran out: copies under way land
+      for (int k = 0; k < a.slots; ++k, row += slots) {
+        if (row < a.rows) mbar_wait_drain(&bars[warp][(slot + k) % a.slots], slot + k < a.slots ? parity : parity ^ 1);
+      }
+    }
+    __syncwarp();
   }
   grid_launch_dependents();
   if (a.partial == nullptr) return;
   float* block_out = a.partial + static_cast<size_t>(blockIdx.x) * 2 * d;
-  float* sums = WARPS > 1 ? block_out : reinterpret_cast<float*>(shared) + static_cast<size_t>(threadIdx.x >> 5) * 2 * d;
-  if constexpr (WARPS == 1) __syncthreads();  // the weights are no longer read
+  float* sums = WARPS > 1 ? block_out : reinterpret_cast<float*>(shared) + static_cast<size_t>(warp) * 2 * d;
+  if constexpr (WARPS == 1) __syncthreads();  // weights and rows are no longer read
 #pragma unroll
   for (int j = 0; j < CPL; ++j) {
 #pragma unroll
@@ -321,47 +454,91 @@ __global__ void __launch_bounds__(1024) norm_finish_kernel(const float* partial,
   else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(s);
 }
 
+int row_warps(int d) { return d <= 1024 ? 1 : kNormWarps; }
+
 unsigned norm_grid(long long rows, int rows_per_block, int blocks) {
   return static_cast<unsigned>(std::max<long long>(1, std::min<long long>((rows + rows_per_block - 1) / rows_per_block, blocks)));
 }
 
+
+// Whether forward blocks walk several rounds of rows.
+bool norm_staged(long long rows, int d) { return rows >= (row_warps(d) == 1 ? 16384 : 2048); }
+
+// Blocks of `kern` an SM holds at once.
+template <class K>
+int blocks_per_sm(K kern, size_t smem) {
+  int n = 0;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kNormThreads, smem) == cudaSuccess && n > 0 ? n : 1;
+}
+
 template <class T, bool VEC, int WARPS, int CPL>
-cudaError_t launch_one(const NormArgs& a, bool backward, unsigned grid, cudaStream_t stream) {
+cudaError_t launch_one(NormArgs a, bool backward, int num_sms, cudaStream_t stream) {
+  constexpr int kPerBlock = kNormWarps / WARPS;
   const size_t weights = static_cast<size_t>(CPL) * 4 * 32 * WARPS * sizeof(float2);
+  if (!backward) {
+    if (norm_staged(a.rows, a.d)) {
+      // One round of blocks: each SM's share of the rows is the same.
+      auto kern = norm_forward_kernel<T, VEC, WARPS, CPL, true>;
+      size_t smem = 2 * weights;
+      int per_warp = 1;  // rows a warp has at work
+      if (norm_ring<VEC, WARPS>()) {
+        const size_t per = static_cast<size_t>(kNormWarps) * a.d * sizeof(T);
+        a.slots = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kForwardSlots, (72 * 1024 - smem) / per)));
+        smem += a.slots * per;
+        if (smem > 32 * 1024) {
+          const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+          if (e != cudaSuccess) return e;
+        }
+      } else if (WARPS == 1) {
+        per_warp = kForwardRows;
+      }
+      const unsigned grid = norm_grid(a.rows, kPerBlock * per_warp, blocks_per_sm(kern, smem) * num_sms);
+      return launch_programmatic(kern, dim3(grid), dim3(kNormThreads), smem, stream, a);
+    }
+    const unsigned grid = norm_grid(a.rows, WARPS == 1 ? kPerBlock * kForwardRows : 1, INT_MAX);
+    return launch_programmatic(norm_forward_kernel<T, VEC, WARPS, CPL, false>, dim3(grid), dim3(kNormThreads), 0, stream, a);
+  }
   const size_t sums = WARPS == 1 && a.partial ? static_cast<size_t>(kNormWarps) * 2 * a.d * 4 : 0;
-  const size_t smem = backward ? std::max(weights, sums) : 2 * weights;
-  auto kern = backward ? norm_backward_kernel<T, VEC, WARPS, CPL> : norm_forward_kernel<T, VEC, WARPS, CPL>;
+  size_t ring = 0;
+  a.slots = 1;
+  if (norm_ring<VEC, WARPS>()) {
+    const size_t per = static_cast<size_t>(kNormWarps) * 2 * a.d * sizeof(T);
+    const size_t room = (sizeof(T) == 4 && CPL > 3 ? 216 : 108) * 1024 - weights;
+    a.slots = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kNormSlots, room / per)));
+    ring = a.slots * per;
+  }
+  const size_t smem = std::max(weights + ring, sums);
+  auto kern = norm_backward_kernel<T, VEC, WARPS, CPL>;
   if (smem > 32 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
   }
+  const unsigned grid = static_cast<unsigned>(norm_backward_blocks(a.rows, a.d, num_sms));
   return launch_programmatic(kern, dim3(grid), dim3(kNormThreads), smem, stream, a);
 }
 
 template <class T, bool VEC>
-cudaError_t launch_width(const NormArgs& a, bool backward, unsigned grid, cudaStream_t stream) {
+cudaError_t launch_width(const NormArgs& a, bool backward, int num_sms, cudaStream_t stream) {
   const int groups = (a.d + 255) / 256;  // groups of eight columns per lane of one warp
-  if (groups <= 1) return launch_one<T, VEC, 1, 1>(a, backward, grid, stream);
-  if (groups <= 2) return launch_one<T, VEC, 1, 2>(a, backward, grid, stream);
-  if (groups <= 3) return launch_one<T, VEC, 1, 3>(a, backward, grid, stream);
-  if (groups <= 4) return launch_one<T, VEC, 1, 4>(a, backward, grid, stream);
-  if (groups <= 8) return launch_one<T, VEC, 8, 1>(a, backward, grid, stream);
-  if (groups <= 16) return launch_one<T, VEC, 8, 2>(a, backward, grid, stream);
-  return launch_one<T, VEC, 8, 4>(a, backward, grid, stream);
+  if (groups <= 1) return launch_one<T, VEC, 1, 1>(a, backward, num_sms, stream);
+  if (groups <= 2) return launch_one<T, VEC, 1, 2>(a, backward, num_sms, stream);
+  if (groups <= 3) return launch_one<T, VEC, 1, 3>(a, backward, num_sms, stream);
+  if (groups <= 4) return launch_one<T, VEC, 1, 4>(a, backward, num_sms, stream);
+  if (groups <= 8) return launch_one<T, VEC, 8, 1>(a, backward, num_sms, stream);
+  if (groups <= 16) return launch_one<T, VEC, 8, 2>(a, backward, num_sms, stream);
+  return launch_one<T, VEC, 8, 4>(a, backward, num_sms, stream);
 }
 
 template <class T>
-cudaError_t launch_type(const NormArgs& a, bool backward, unsigned grid, cudaStream_t stream) {
+cudaError_t launch_type(const NormArgs& a, bool backward, int num_sms, cudaStream_t stream) {
   const auto ok = [&](const void* p, long long stride, size_t es) {
     return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (stride * es) % 16 == 0);
   };
   const size_t es = sizeof(T), ws = a.w32 ? 4 : es;
   const bool vec = a.d % 8 == 0 && ok(a.x, a.x_stride, es) && ok(a.y, a.y_stride, es) && ok(a.dy, a.dy_stride, es) &&
                    ok(a.dx, a.dx_stride, es) && ok(a.weight, 0, ws) && ok(a.bias, 0, ws);
-  return vec ? launch_width<T, true>(a, backward, grid, stream) : launch_width<T, false>(a, backward, grid, stream);
+  return vec ? launch_width<T, true>(a, backward, num_sms, stream) : launch_width<T, false>(a, backward, num_sms, stream);
 }
-
-int row_warps(int d) { return d <= 1024 ? 1 : kNormWarps; }
 
 }  // namespace
 
@@ -371,18 +548,16 @@ int norm_backward_blocks(long long rows, int d, int num_sms) {
 
 cudaError_t norm_launch(const NormArgs& a, int dtype, bool backward, int num_sms, cudaStream_t stream) {
   if (a.d < 1 || a.d > kNormMaxWidth || a.rows < 1) return cudaErrorInvalidValue;
-  const unsigned grid = backward ? static_cast<unsigned>(norm_backward_blocks(a.rows, a.d, num_sms))
-                                 : norm_grid(a.rows, kNormWarps / row_warps(a.d), 16 * num_sms);
   cudaError_t e;
   switch (dtype) {
-    case kSrcF32: e = launch_type<float>(a, backward, grid, stream); break;
-    case kSrcF16: e = launch_type<__half>(a, backward, grid, stream); break;
-    case kSrcBF16: e = launch_type<__nv_bfloat16>(a, backward, grid, stream); break;
+    case kSrcF32: e = launch_type<float>(a, backward, num_sms, stream); break;
+    case kSrcF16: e = launch_type<__half>(a, backward, num_sms, stream); break;
+    case kSrcBF16: e = launch_type<__nv_bfloat16>(a, backward, num_sms, stream); break;
     default: return cudaErrorInvalidValue;
   }
   if (e != cudaSuccess || !backward || a.partial == nullptr) return e;
   return launch_programmatic(norm_finish_kernel, dim3(static_cast<unsigned>((2 * a.d + 31) / 32)), dim3(1024), 0, stream,
-                             static_cast<const float*>(a.partial), static_cast<int>(grid), a.d, a.dweight, a.dbias,
+                             static_cast<const float*>(a.partial), norm_backward_blocks(a.rows, a.d, num_sms), a.d, a.dweight, a.dbias,
                              a.w32 ? static_cast<int>(kSrcF32) : dtype);
 }
 

@@ -95,15 +95,6 @@ __device__ __forceinline__ float clamped_norm(const Pair (&u)[CPL][4]) {
   return fmaxf(sqrtf(warp_sum(pair_total(ss))), 1e-12f);
 }
 
-// Copies `bytes` (a multiple of 16, both addresses 16-byte aligned) to shared memory,
-// completion on an mbarrier that expects them.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 // Group j of a staged row (zeros behind the row, which only the last group can reach).
 template <int CPL>
 __device__ __forceinline__ Raw8<__half> staged(const uint8_t* row, int d_pad, int lane, int j) {

@@ -95,6 +95,24 @@ def test_layer_norm(cvs, dtype, rows, d):
                randn(d, dtype=t, seed=3), randn(rows, d, dtype=t, seed=4))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,d", [(16384, 8), (16391, 96), (20000, 768), (18001, 1024), (17000, 65), (2500, 1032)])
+def test_layer_norm_many_rows(cvs, dtype, rows, d):
+    """Enough rows for the kernels that walk them through rings of row buffers."""
+    t = DTYPES[dtype]
+    check_norm(cvs, randn(rows, d, dtype=t, seed=1, scale=2.0, shift=0.5), randn(d, dtype=t, seed=2, shift=1.0),
+               randn(d, dtype=t, seed=3), randn(rows, d, dtype=t, seed=4))
+
+
+def test_layer_norm_many_strided_rows(cvs):
+    x = strided(randn(17000, 320, dtype=torch.float16, seed=1), "rows")
+    dy = strided(randn(17000, 320, dtype=torch.float16, seed=4), "rows")
+    check_norm(cvs, x, randn(320, dtype=torch.float32, seed=2), None, dy)
+    row = randn(1, 320, dtype=torch.float16, seed=5)
+    y = cvs.layer_norm(row.expand(17000, 320))  # every row the same one in memory
+    assert torch.equal(y, cvs.layer_norm(row).expand(17000, 320))
+
+
 @pytest.mark.parametrize("kind", ["rows", "odd", "columns"])
 @pytest.mark.parametrize("d", [64, 391])
 def test_layer_norm_strides(cvs, kind, d):
