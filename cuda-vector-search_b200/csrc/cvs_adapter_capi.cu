@@ -286,6 +286,20 @@ cvs_status cvs_layer_norm_backward(const void* dy, int64_t dy_stride, const void
   return e == cudaSuccess ? CVS_OK : cuda_fail(e, "layer norm backward launch");
 }
 
+cvs_status cvs_align_rows(const void* src, int64_t src_stride, int dtype, int64_t rows, int cols, void* dst,
+                          int64_t dst_stride, void* stream) {
+  if (dtype != CVS_F16 && dtype != CVS_BF16) return fail(CVS_ERR_INVALID_ARGUMENT, "float16 or bfloat16 (got dtype %d)", dtype);
+  if (rows < 0 || cols < 1) return fail(CVS_ERR_INVALID_ARGUMENT, "bad matrix shape [%lld][%d]", (long long)rows, cols);
+  if (rows == 0) return CVS_OK;
+  if (!src || (rows > 1 && src_stride < 0)) return fail(CVS_ERR_INVALID_ARGUMENT, "bad source");
+  cvs_status st = check_operand(dst, dst_stride, cols, "dst");
+  if (st != CVS_OK) return st;
+  DeviceInfo dev;
+  if ((st = device_info(&dev)) != CVS_OK) return st;
+  const cudaError_t e = pad_rows_launch(src, rows, cols, src_stride, dst, dst_stride, dev.sms, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CVS_OK : cuda_fail(e, "row alignment launch");
+}
+
 cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
                       const void* residual, int64_t residual_stride, int activation, int dtype, int64_t m, int n,
                       int k, void* y, int64_t y_stride, void* z, int64_t z_stride, void* stream) {

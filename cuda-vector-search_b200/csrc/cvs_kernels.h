@@ -278,6 +278,9 @@ struct LinearSmallArgs {
 };
 cudaError_t linear_small_launch(const LinearSmallArgs& a, cudaStream_t stream);
 
+cudaError_t pad_rows_launch(const void* src, long long rows, int cols, long long ld_src, void* dst, long long ld_dst,
+                            int num_sms, cudaStream_t stream);
+
 struct LinearDzArgs {
   const void* dy;
   const void* z;     // null: no activation

@@ -24,6 +24,7 @@
 #include "cvs_kernels.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace cvs {
 
@@ -343,7 +344,6 @@ template <int N>
 __device__ __forceinline__ void tma_store_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // This thread's writes to shared memory are visible to the copies issued after it.
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(GemmShape<CG, BN>::kThreads, 1)
       mbar_wait_drain(sh.rfull(ew, 0), rphase & 1);
       mbar_wait_drain(sh.rfull(ew, 1), rphase >> 1);
     }
-    if (lane == 0) tma_store_wait_all();
+    if (lane == 0) tma_store_wait_read<0>();
     __syncwarp();
   }
 
@@ -925,12 +925,56 @@ __global__ void __launch_bounds__(256) linear_finish_kernel(const LinearFinishAr
   }
 }
 
+// ---------------------------------------------------------------------------
+// Operands the tensor-memory accelerator cannot address
+// ---------------------------------------------------------------------------
+// Copies rows of any alignment into rows of whole 16-byte units: one warp per row and 256
+// columns at a time, eight two-byte loads under way per lane, consecutive over the warp,
+// regrouped through shared memory into 16-byte stores.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* src, long long rows, int cols, long long ld_src,
+                                                       uint16_t* dst, long long ld_dst) {
+  __shared__ __align__(16) uint16_t buf[8][256];
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = (cols + 255) / 256;
+  const long long items = rows * chunks;
+  for (long long i = static_cast<long long>(blockIdx.x) * 8 + warp; i < items; i += static_cast<long long>(gridDim.x) * 8) {
+    const long long row = i / chunks;
+    const int c0 = static_cast<int>(i - row * chunks) * 256;
+    const uint16_t* p = src + row * ld_src + c0;
+    uint16_t v[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) v[t] = c0 + 32 * t + lane < cols ? p[32 * t + lane] : static_cast<uint16_t>(0);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) buf[warp][32 * t + lane] = v[t];
+    __syncwarp();
+    const int c = c0 + lane * 8;
+    if (c < ld_dst)
+      *reinterpret_cast<uint4*>(dst + row * ld_dst + c) = *reinterpret_cast<const uint4*>(&buf[warp][lane * 8]);
+    __syncwarp();
+  }
+}
+
+// Sets a kernel's dynamic shared memory limit, once per device.
+template <class K>
+cudaError_t allow_smem(K kern, int smem, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <int CG, int BN>
 cudaError_t gemm_launch_one(const GemmMaps& maps, const GemmArgs& a, int ctas, cudaStream_t stream) {
   using S = GemmShape<CG, BN>;
   constexpr int smem = S::kTotal + 1024;
   auto kern = gemm_kernel<CG, BN>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
@@ -965,6 +1009,14 @@ cudaError_t linear_small_launch(const LinearSmallArgs& a, cudaStream_t stream) {
   if (a.m <= 4) return launch_programmatic(linear_small_kernel<4>, grid, dim3(256), 0, stream, a);
   if (a.m <= kLinearSmallRows) return launch_programmatic(linear_small_kernel<8>, grid, dim3(256), 0, stream, a);
   return cudaErrorInvalidValue;
+}
+
+cudaError_t pad_rows_launch(const void* src, long long rows, int cols, long long ld_src, void* dst, long long ld_dst,
+                            int num_sms, cudaStream_t stream) {
+  const long long items = rows * ((cols + 255) / 256);
+  const dim3 grid(static_cast<unsigned>(std::max<long long>(1, std::min<long long>((items + 7) / 8, 8LL * num_sms))));
+  return launch_programmatic(pad_rows_kernel, grid, dim3(256), 0, stream, static_cast<const uint16_t*>(src), rows, cols,
+                             ld_src, static_cast<uint16_t*>(dst), ld_dst);
 }
 
 int linear_dz_parts(long long m, int n, int num_sms) {

@@ -55,9 +55,12 @@ Tensor with_tiles(const Tensor& t) {
   const bool ok = reinterpret_cast<std::uintptr_t>(t.data_ptr()) % 16 == 0 && (t.stride(1) == 1 || t.size(1) <= 1) &&
                   (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1)));
   if (ok) return t;
-  Tensor out = torch::empty({t.size(0), pad8(t.size(1))}, t.options()).narrow(1, 0, t.size(1));
-  out.copy_(t);
-  return out;
+  const Tensor src = with_rows(t);
+  const Tensor out = torch::empty({t.size(0), pad8(t.size(1))}, t.options());
+  check(cvs_align_rows(src.data_ptr(), row_stride(src), code(src), src.size(0), static_cast<int>(src.size(1)), out.data_ptr(),
+                       out.size(1), stream_of(src)),
+        "linear");
+  return out.narrow(1, 0, t.size(1));
 }
 
 void check_device(const Tensor& t, const char* name, const Tensor& first) {
@@ -195,6 +198,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
 // ---- linear -----------------------------------------------------------------
 struct LinearOut {
   Tensor y, z;
+  Tensor x, w;  // as the product read them (copies where their rows were not aligned)
 };
 
 LinearOut linear_forward(const Tensor& x_in, const Tensor& w_in, const Tensor& bias_in, const Tensor& residual_in,
@@ -215,6 +219,8 @@ LinearOut linear_forward(const Tensor& x_in, const Tensor& w_in, const Tensor& b
                    activation, code(x), m, static_cast<int>(n), static_cast<int>(k), out.y.data_ptr(), n,
                    keep ? out.z.data_ptr() : nullptr, keep ? pad8(n) : 0, stream_of(x)),
         "linear");
+  out.x = x;
+  out.w = w;
   return out;
 }
 
@@ -225,7 +231,9 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
     // z is only read by an activation's derivative.
     const bool keep = activation != CVS_ACT_NONE;
     LinearOut out = linear_forward(x, weight, or_undefined(bias), or_undefined(residual), static_cast<int>(activation), keep);
-    ctx->save_for_backward({x, weight, out.z});
+    // Where the product read aligned copies, the backward pass reads them again instead
+    // of making its own (more than CVS_LINEAR_SMALL_ROWS rows; else the inputs as they are).
+    ctx->save_for_backward({out.x, out.w, out.z});
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["bias"] = given(bias);
     ctx->saved_data["residual"] = given(residual);

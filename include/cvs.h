@@ -235,6 +235,14 @@ cvs_status cvs_layer_norm_backward(const void* dy, int64_t dy_stride, const void
                                    void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Copies half-precision rows of any alignment into rows that cvs_linear and
+ * cvs_linear_backward accept: dst 16-byte aligned, dst_stride a multiple of 8 and
+ * at least cols. Columns cols .. dst_stride-1 of dst may be written with zeros.
+ */
+cvs_status cvs_align_rows(const void* src, int64_t src_stride, int dtype, int64_t rows, int cols, void* dst,
+                          int64_t dst_stride, void* stream);
+
+/*
  * y[m][n] = act(x[m][k] . w[n][k]^T + bias) + residual, dtype CVS_F16 or CVS_BF16
  * for every operand. bias [n] and residual [m][n] may be NULL. z, unless NULL,
  * receives x . w^T + bias as fp16 (also for CVS_BF16) for cvs_linear_backward:
