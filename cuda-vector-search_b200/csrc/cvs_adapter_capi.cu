@@ -124,6 +124,20 @@ Tile pick_tile(int64_t m, int64_t n, int sms) {
   return best;
 }
 
+// CTAs that share a 128 x 64 tile's K dimension (0: the persistent kernel). Eight as long
+// as one round of SMs holds them, four as long as two rounds do (two CTAs fit on an SM),
+// two where one round does or K is long. Measured (us, persistent / 2 / 4 / 8): 64 rows,
+// 768 -> 1536 (24 tiles): 7.7 / 6.6 / 5.2 / 5.7; 16 rows, 1536 -> 768 (12): 10.2 / 7.5 /
+// 5.5 / 4.8; 32 rows, 4096 -> 4096 (64): 19.4 / 12.5 / 9.9 / 15.1; 512 rows, 768 -> 1536
+// (96): 8.5 / 9.0 / 12.2 / 17.3; 256 rows, 4096 -> 4096 (128): 20.9 / 16.9 / 21.7 / 31.7.
+int pick_splits(int64_t m, int64_t n, int64_t k, int sms) {
+  const int64_t tiles = ceil_div(m, 128) * ceil_div(n, 64), kblocks = ceil_div(k, 64);
+  if (8 * tiles <= sms && kblocks >= 6) return 8;
+  if (4 * tiles <= 2 * sms && kblocks >= 4) return 4;
+  if (2 * tiles <= (kblocks >= 32 ? 2 * sms : sms) && kblocks >= 2) return 2;
+  return 0;
+}
+
 void set_shape(GemmProblem* p, const Tile& t, int64_t m, int64_t n, int64_t k, int splits) {
   p->m = static_cast<int>(m);
   p->n = static_cast<int>(n);
@@ -314,7 +328,11 @@ cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_
   DeviceInfo dev;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (m <= kLinearSmallRows) {
+  // Up to two rows the CUDA cores stream the weights fastest (768 -> 1536, one, two, four,
+  // eight rows: 2.4, 3.3, 5.0, 8.6 us, against 5.0 us on the tensor cores at each); rows
+  // of any alignment stay there a little longer rather than have the weights copied.
+  const bool tiles = mappable(x, m > 1 ? x_stride : ceil_div(k, 8) * 8, k) && mappable(w, w_stride, k);
+  if (m <= 2 || (m <= kLinearSmallRows && !tiles)) {
     if ((m > 1 && x_stride < 0) || w_stride < k)
       return fail(CVS_ERR_INVALID_ARGUMENT, "bad row stride");
     if ((st = device_info(&dev)) != CVS_OK) return st;
@@ -342,6 +360,32 @@ cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_
   if ((st = check_operand(x, x_stride, k, "x")) != CVS_OK) return st;
   if ((st = check_operand(w, w_stride, k, "w")) != CVS_OK) return st;
   if ((st = device_info(&dev)) != CVS_OK) return st;
+  if (const int splits = pick_splits(m, n, k, dev.sms)) {
+    SplitArgs a{};
+    a.m = static_cast<int>(m);
+    a.n = n;
+    a.tiles_m = static_cast<int>(ceil_div(m, 128));
+    a.kblocks = static_cast<int>(ceil_div(k, 64));
+    a.kper = static_cast<int>(ceil_div(a.kblocks, splits));
+    a.a_rows = static_cast<int>(std::min<int64_t>(128, (m + 7) / 8 * 8));
+    a.act = activation;
+    a.bf16 = dtype == CVS_BF16;
+    a.bias = bias;
+    a.residual = residual;
+    a.out = y;
+    a.z = z;
+    a.ld_res = residual_stride;
+    a.ld_out = y_stride;
+    a.ld_z = z_stride;
+    a.vec_res = aligned16(residual) && residual_stride % 8 == 0;
+    a.vec_out = aligned16(y) && y_stride % 8 == 0;
+    a.err = dev.err;
+    CUtensorMap amap, bmap;
+    if ((st = operand_map(&amap, {x, x_stride, false}, dtype, m, k, a.a_rows)) != CVS_OK) return st;
+    if ((st = operand_map(&bmap, {w, w_stride, false}, dtype, n, k, 64)) != CVS_OK) return st;
+    e = split_launch(splits, amap, bmap, a, a.tiles_m * static_cast<int>(ceil_div(n, 64)), s);
+    return e == cudaSuccess ? CVS_OK : cuda_fail(e, "linear launch");
+  }
   const Tile t = pick_tile(m, n, dev.sms);
   GemmMaps maps{};
   if ((st = operand_map(&maps.a[0], {x, x_stride, false}, dtype, m, k, 128)) != CVS_OK) return st;

@@ -264,6 +264,25 @@ struct GemmMaps {
 // Tile shapes: cg CTAs (128 rows each) x bn columns.
 cudaError_t gemm_launch(int cg, int bn, const GemmMaps& maps, const GemmArgs& a, int ctas, cudaStream_t stream);
 
+// One product of few 128 x 64 tiles, its K slices shared by the 2, 4 or 8 CTAs of a
+// cluster. amap: boxes of 64 columns x a_rows rows, bmap: 64 x 64.
+struct SplitArgs {
+  int m, n;
+  int tiles_m;
+  int kblocks, kper;     // slices of 64 along K, per CTA
+  int a_rows;
+  int act, bf16;
+  const void* bias;
+  const void* residual;
+  void* out;
+  void* z;
+  long long ld_res, ld_out, ld_z;
+  int vec_res, vec_out;  // rows 16-byte aligned
+  int* err;
+};
+cudaError_t split_launch(int splits, const CUtensorMap& amap, const CUtensorMap& bmap, const SplitArgs& a, int tiles,
+                         cudaStream_t stream);
+
 struct LinearSmallArgs {
   const void* x;
   const void* w;

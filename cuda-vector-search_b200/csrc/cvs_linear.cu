@@ -156,6 +156,16 @@ __device__ __forceinline__ uint16_t half_bits(float v, bool bf16) {
   return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
+// Eight halves of a row from column c on (columns outside read as zero).
+__device__ __forceinline__ uint4 load_unit8(const uint16_t* p, int c, int n, bool vec) {
+  if (vec && c + 8 <= n) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+    if (c + t < n) w[t / 2] |= static_cast<uint32_t>(p[t]) << (16 * (t & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // ---------------------------------------------------------------------------
 // tcgen05 product
 // ---------------------------------------------------------------------------
@@ -692,18 +702,201 @@ __global__ void __launch_bounds__(GemmShape<CG, BN>::kThreads, 1)
     __syncwarp();
   }
 
-  // The next kernel may be scheduled from here on. Not earlier: the kernels of this
-  // file trigger only behind their last read of global memory, so that no later
-  // kernel of a chain is resident (its L1 cache in use) while an input is still
-  // being read whose memory the chain reuses for another kernel's result.
-  grid_launch_dependents();
   tc_fence_before();
   __syncthreads();
+  // The next kernel may be scheduled from here on. Not earlier: no kernel of a forward
+  // pass triggers before all its warps' last read of global memory, so that no later
+  // kernel of a chain is resident (its L1 cache in use) while an input is still being
+  // read whose memory the chain reuses for another kernel's result.
+  grid_launch_dependents();
   if constexpr (CG == 2) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
     if constexpr (CG == 2) tmem_dealloc_pair(tmem_base, S::kTmemCols);
     else tmem_dealloc(tmem_base, S::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few tiles: K split over a cluster
+// ---------------------------------------------------------------------------
+// Where 128 x 64 tiles do not fill the GPU, the S CTAs of a cluster share one tile's K
+// dimension. Each sends its fp32 sums of column slice c to CTA c through distributed
+// shared memory; after one cluster barrier CTA c adds the S parts in order and finishes
+// its 64 / S columns (bias, activation, residual). No workspace, one launch, the same
+// result every run.
+constexpr int kSplitN = 64;
+constexpr int kSplitStages = 3;
+constexpr int kSplitThreads = 192;
+
+struct SplitLayout {
+  static constexpr int kABytes = kGemmM * kGemmK * 2, kBBytes = kSplitN * kGemmK * 2;
+  static constexpr int kStage = kABytes + kBBytes;
+  static constexpr int kParts = kSplitStages * kStage;              // offset of the received parts
+  static constexpr int kBars = kParts + kGemmM * kSplitN * 4;
+  static constexpr int kTotal = kBars + 8 * (2 * kSplitStages + 1) + 16;
+};
+
+template <int S>
+__global__ void __launch_bounds__(kSplitThreads)
+    split_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                 const __grid_constant__ SplitArgs a) {
+  using L = SplitLayout;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + L::kBars);
+  uint64_t* empty = full + kSplitStages;
+  uint64_t* done = empty + kSplitStages;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(done + 1) + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int tile = static_cast<int>(blockIdx.x) / S;
+  const int mt = tile % a.tiles_m, nt = tile / a.tiles_m;
+  const int k0 = static_cast<int>(rank) * a.kper, k1 = min(a.kblocks, k0 + a.kper);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSplitStages; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    mbar_init(done, 1);
+    *abort = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&amap);
+    tma_prefetch_desc(&bmap);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, kSplitN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  grid_dependency_wait();
+  if (warp == 0) {
+    if (elect_one_lane()) {
+      int it = 0;
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int s = it % kSplitStages;
+        if (!mbar_wait(empty + s, ((it / kSplitStages) & 1) ^ 1, abort, a.err, 44)) {
+          for (int j = max(0, it - kSplitStages); j < it; ++j)
+            mbar_wait_drain(full + j % kSplitStages, (j / kSplitStages) & 1);
+          break;
+        }
+        // A's box ends with the last row (rows below it in the tile keep what they had:
+        // they only reach accumulator rows that nobody stores).
+        mbar_arrive_expect_tx(full + s, static_cast<uint32_t>(a.a_rows) * (kGemmK * 2) + L::kBBytes);
+        tma_load_tile(base + s * L::kStage, &amap, full + s, kb * kGemmK, mt * kGemmM);
+        tma_load_tile(base + s * L::kStage + L::kABytes, &bmap, full + s, kb * kGemmK, nt * kSplitN);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one_lane()) {
+      const uint32_t idesc = gemm_idesc(kGemmM, kSplitN, a.bf16 != 0, false, false);
+      int it = 0;
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int s = it % kSplitStages;
+        if (!mbar_wait(full + s, (it / kSplitStages) & 1, abort, a.err, 45)) break;
+        tc_fence_after();
+        const uint32_t sa = smem_u32(base + s * L::kStage), sb = sa + L::kABytes;
+#pragma unroll
+        for (int kk = 0; kk < kGemmK / 16; ++kk)
+          tc_mma_f16(tmem, gemm_desc(sa + kk * 32, false), gemm_desc(sb + kk * 32, false), idesc, (it | kk) != 0 ? 1u : 0u);
+        tc_commit(empty + s);
+      }
+      tc_commit(done);
+      mbar_wait_drain(done, 0);
+    }
+    __syncwarp();
+  } else {
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, abort, a.err, 46));
+    tc_fence_after();
+    const uint32_t parts = smem_u32(base + L::kParts);
+    constexpr int kQ = kSplitN / S / 4;  // float4 groups per slice
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t r[32];
+      if (ok && k0 < k1) {
+        tmem_ld32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + 32 * h, r);
+        tmem_wait_ld32(r);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = 0u;
+      }
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const int group = 8 * h + g;  // columns 4 group .. 4 group + 3
+        const uint32_t to = map_to_rank(parts + ((rank * kQ + group % kQ) * kGemmM + row) * 16, group / kQ);
+        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(r[4 * g]), "r"(r[4 * g + 1]),
+                     "r"(r[4 * g + 2]), "r"(r[4 * g + 3])
+                     : "memory");
+      }
+    }
+  }
+  tc_fence_before();
+  cluster_sync_all();  // every part has arrived; nobody writes to another CTA after this
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kSplitN);
+  }
+  if (warp < 2) return;
+  const int row = (warp & 3) * 32 + lane;
+  const long long out_row = static_cast<long long>(mt) * kGemmM + row;
+  if (out_row >= a.m) return;
+  const bool bf16 = a.bf16 != 0;
+  constexpr int kQ = kSplitN / S / 4;
+  const float4* parts = reinterpret_cast<const float4*>(base + L::kParts);
+#pragma unroll
+  for (int e = 0; e < kQ / 2; ++e) {
+    const int col = nt * kSplitN + static_cast<int>(rank) * (kSplitN / S) + 8 * e;
+    if (col >= a.n) break;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const float4 lo = parts[(s * kQ + 2 * e) * kGemmM + row], hi = parts[(s * kQ + 2 * e + 1) * kGemmM + row];
+      v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+      v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+    }
+    if (a.bias) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < a.n) v[i] += half_at(a.bias, col + i, bf16);
+    }
+    if (a.z) {
+      float kept[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) kept[i] = a.act == kActRelu && v[i] > 0.f ? fmaxf(v[i], 6e-8f) : v[i];
+      // z's rows are whole 16-byte units.
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.z) + out_row * a.ld_z + col) =
+          make_uint4(pack2(kept[0], kept[1], false), pack2(kept[2], kept[3], false), pack2(kept[4], kept[5], false),
+                     pack2(kept[6], kept[7], false));
+    }
+    act_values(v, a.act);
+    if (a.residual) {
+      const uint4 q = load_unit8(static_cast<const uint16_t*>(a.residual) + out_row * a.ld_res + col, col, a.n, a.vec_res != 0);
+      const uint32_t qs[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2(qs[i], bf16);
+        v[2 * i] += f.x;
+        v[2 * i + 1] += f.y;
+      }
+    }
+    uint16_t* out = static_cast<uint16_t*>(a.out) + out_row * a.ld_out + col;
+    if (a.vec_out && col + 8 <= a.n) {
+      *reinterpret_cast<uint4*>(out) = make_uint4(pack2(v[0], v[1], bf16), pack2(v[2], v[3], bf16), pack2(v[4], v[5], bf16),
+                                                  pack2(v[6], v[7], bf16));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < a.n) out[i] = half_bits(v[i], bf16);
+    }
   }
 }
 
@@ -775,16 +968,6 @@ __global__ void __launch_bounds__(256) linear_small_kernel(const LinearSmallArgs
 constexpr int kDzCols = 256;  // columns per block: one warp reads 32 x 16 bytes of a row
 constexpr int kDzWarps = 8;
 constexpr int kDzRows = 4;    // rows a thread has in flight
-
-// Eight halves of a row from column c on (columns outside read as zero).
-__device__ __forceinline__ uint4 load_unit8(const uint16_t* p, int c, int n, bool vec) {
-  if (vec && c + 8 <= n) return *reinterpret_cast<const uint4*>(p);
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int t = 0; t < 8; ++t)
-    if (c + t < n) w[t / 2] |= static_cast<uint32_t>(p[t]) << (16 * (t & 1));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
 // dz = dy act'(z) in the rows' type (dz null: nothing to write, no activation), and
 // the block's share of every column's sum, in fp32 from the unrounded dz. Bound by
@@ -1000,6 +1183,42 @@ cudaError_t gemm_launch(int cg, int bn, const GemmMaps& maps, const GemmArgs& a,
   if (cg == 1 && bn == 128) return gemm_launch_one<1, 128>(maps, a, ctas, stream);
   if (cg == 1 && bn == 64) return gemm_launch_one<1, 64>(maps, a, ctas, stream);
   return cudaErrorInvalidValue;
+}
+
+namespace {
+template <int S>
+cudaError_t split_launch_one(const CUtensorMap& amap, const CUtensorMap& bmap, const SplitArgs& a, int ctas, cudaStream_t stream) {
+  constexpr int smem = SplitLayout::kTotal + 1024;
+  auto kern = split_kernel<S>;
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_smem(kern, smem, allowed);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = S;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, amap, bmap, a);
+}
+}  // namespace
+
+cudaError_t split_launch(int splits, const CUtensorMap& amap, const CUtensorMap& bmap, const SplitArgs& a, int tiles,
+                         cudaStream_t stream) {
+  switch (splits) {
+    case 2: return split_launch_one<2>(amap, bmap, a, 2 * tiles, stream);
+    case 4: return split_launch_one<4>(amap, bmap, a, 4 * tiles, stream);
+    case 8: return split_launch_one<8>(amap, bmap, a, 8 * tiles, stream);
+    default: return cudaErrorInvalidValue;
+  }
 }
 
 cudaError_t linear_small_launch(const LinearSmallArgs& a, cudaStream_t stream) {

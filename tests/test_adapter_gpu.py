@@ -226,6 +226,18 @@ def test_linear(cvs, dtype, m, k, n):
                  randn(m, n, dtype=t, seed=4))
 
 
+# Few tiles: a cluster of 2, 4 or 8 CTAs shares K; rings that go round; K that does not
+# divide among them (CTAs without a slice); one tile and several rounds of tiles.
+@pytest.mark.parametrize("m,k,n", [(3, 128, 64), (12, 320, 8), (40, 4096, 520), (200, 4104, 640), (9, 391, 65), (70, 448, 2000),
+                                   (130, 2048, 3000), (500, 256, 64), (16, 64, 64)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_linear_shared_k(cvs, m, k, n, residual):
+    t = torch.bfloat16
+    check_linear(cvs, randn(m, k, dtype=t, seed=1), randn(n, k, dtype=t, seed=2, scale=k**-0.5), randn(n, dtype=t, seed=3),
+                 ("relu", "silu", "gelu", "none")[m % 4], randn(m, n, dtype=t, seed=5) if residual else None,
+                 randn(m, n, dtype=t, seed=4))
+
+
 @pytest.mark.parametrize("activation", ["none", "relu", "gelu", "silu"])
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("m", [3, 150, 700])
