@@ -456,7 +456,8 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
   const bool dy_tiles = aligned16(dy) && dy_stride % 8 == 0 && dy_stride >= n;  // TMA can read dy itself
   Operand dz{dy, dy_stride, false};
   if (act || !dy_tiles) dz = {base + plan.dz_offset, plan.dz_stride, false};
-  if (act || dbias || (!dy_tiles && (dx || dw))) {
+  const bool needs_dz = act || (!dy_tiles && (dx || dw));
+  const auto launch_dz = [&]() {
     LinearDzArgs a{};
     a.dy = dy;
     a.ld_dy = dy_stride;
@@ -470,8 +471,9 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
     a.n = n;
     a.act = activation;
     a.bf16 = bf16;
-    if ((e = linear_dz_launch(a, plan.db_parts, s)) != cudaSuccess) return cuda_fail(e, "linear backward launch");
-  }
+    return linear_dz_launch(a, plan.db_parts, s);
+  };
+  if (needs_dz && (e = launch_dz()) != cudaSuccess) return cuda_fail(e, "linear backward launch");
   const Tile& t = plan.tile;
   if (dx || dw) {
     GemmMaps maps{};
@@ -508,6 +510,8 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
     if ((e = gemm_launch(t.cg, t.bn, maps, a, grid_ctas(t, work, dev.sms), s)) != cudaSuccess)
       return cuda_fail(e, "linear backward launch");
   }
+  // Without dz only dbias needs dy's columns: after the products, which leave part of dy in L2.
+  if (!needs_dz && dbias && (e = launch_dz()) != cudaSuccess) return cuda_fail(e, "linear backward launch");
   LinearFinishArgs f{};
   f.db_partial = reinterpret_cast<const float*>(base + plan.db_offset);
   f.db_parts = plan.db_parts;

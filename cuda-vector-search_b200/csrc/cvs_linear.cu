@@ -631,7 +631,11 @@ __global__ void __launch_bounds__(GemmShape<CG, BN>::kThreads, 1)
             __syncwarp();
           }
         }
-        if (!live) continue;
+        if (!live) {
+          // An empty group, so that "all but the last group" still means the other buffer's.
+          if ((c & 1) != 0 && lane == 0) tma_store_commit();
+          continue;
+        }
         float v[32];
         if (p.bias) {
           bias_s[lane] = bias_r[c];

@@ -337,6 +337,8 @@ class Index:
         if reduction not in ("mean", "sum"):
             raise ValueError("reduction must be 'mean' or 'sum'")
         q = self._query_tensor(queries)
+        if reference is not None:
+            reference = self._query_tensor(reference)
         rejected = self._ids(rejected)
         if rejected.dim() == 1:
             rejected = rejected[:, None]

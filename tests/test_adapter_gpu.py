@@ -256,6 +256,21 @@ def test_linear_strides(cvs, kind, m, k, n):
                  strided(randn(m, n, dtype=t, seed=4), kind))
 
 
+@pytest.mark.parametrize("n", [64, 320, 832])
+@pytest.mark.parametrize("activation", ["none", "gelu"])
+def test_linear_narrow_last_tiles(cvs, n, activation):
+    """Tiles whose second half lies outside the matrix, many per CTA: every block of the
+    result, and of the kept pre-activation, leaves before its buffer is written again."""
+    t = torch.float16
+    x, w = randn(60000, 64, dtype=t, seed=1), randn(n, 64, dtype=t, seed=2, scale=0.2)
+    want, z, _, scale = oracle.linear(x, w, None, activation, None)
+    with torch.no_grad():
+        oracle.close(cvs.linear(x, w, activation=activation), want, 40 * E * scale + 16 * E * z.abs())
+    wr = w.clone().requires_grad_()
+    y = cvs.linear(x, wr, activation=activation)
+    oracle.close(y, want, 40 * E * scale + 16 * E * z.abs())
+
+
 def test_linear_broadcast_operands(cvs):
     """Rows that are one row in memory: an expanded input, residual and upstream
     gradient; the shared row's gradient is the sum over its uses."""
@@ -418,6 +433,14 @@ def test_preference(cvs, metric, dtype, b, r, d):
 def test_preference_one_rejected_as_a_vector(cvs):
     index = make_index(cvs, 300, 128, "cosine")
     check_preference(cvs, index, randn(10, 128, dtype=torch.float32, seed=1), ids(300, 10, seed=3), ids(300, 10, seed=4))
+
+
+def test_preference_of_one_query_given_as_a_vector(cvs):
+    index = make_index(cvs, 300, 128, "cosine")
+    q, ref = randn(1, 128, dtype=torch.float32, seed=1), randn(1, 128, dtype=torch.float32, seed=2)
+    a = index.preference_loss(q, [3], [4], reference=ref)
+    b = index.preference_loss(q[0], torch.tensor([3]), [[4]], reference=ref[0])
+    assert torch.equal(a, b)
 
 
 def test_preference_absent_rows_only(cvs):
