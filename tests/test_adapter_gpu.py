@@ -696,3 +696,62 @@ def test_second_derivatives_are_refused(cvs):
     y = cvs.layer_norm(x)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+# ---- sizes past 32 bits -----------------------------------------------------------
+def test_more_than_two_to_the_31_elements(cvs):
+    """Inputs, results and gradients of more than 2^31 elements: their last rows (and
+    first) agree with the same rows computed alone."""
+    t = torch.float16
+    d = 1024
+    rows = (1 << 31) // d + 777
+    x = torch.zeros(rows, d, dtype=t, device="cuda")
+    x[:100] = randn(100, d, dtype=t, seed=1)
+    x[-100:] = randn(100, d, dtype=t, seed=2)
+    w = randn(d, dtype=t, seed=3)
+    y = cvs.layer_norm(x, w)
+    assert torch.equal(y[-100:], cvs.layer_norm(x[-100:], w)) and torch.equal(y[:100], cvs.layer_norm(x[:100], w))
+    assert (y[100:-100][:: 1 << 12] == 0).all()
+    del y
+    w2 = randn(24, d, dtype=t, seed=4, scale=0.03)
+    y = cvs.linear(x, w2)  # the largest input
+    oracle.close(y[-100:], x[-100:].double() @ w2.double().T, 200 * E * (x[-100:].double().abs() @ w2.double().abs().T))
+    del y
+    xr = x.requires_grad_()
+    yn = cvs.layer_norm(xr, w)
+    dy = torch.zeros_like(x)
+    dy[-100:] = randn(100, d, dtype=t, seed=5)
+    (dx,) = torch.autograd.grad(yn, xr, dy)
+    _, want, _, _, _ = oracle.layer_norm(x[-100:].detach(), w, None, 1e-5, dy[-100:])
+    oracle.close(dx[-100:], want, 2.0**-16 * want.abs() + 2.0**-18)
+    assert (dx[:-100][:: 1 << 12] == 0).all()
+
+
+def test_linear_result_past_32_bits(cvs):
+    t = torch.bfloat16
+    n = 520
+    m = (1 << 31) // n + 300
+    x, w, b = randn(m, 64, dtype=t, seed=1), randn(n, 64, dtype=t, seed=2, scale=0.1), randn(n, dtype=t, seed=3)
+    y = cvs.linear(x, w, b, activation="gelu")
+    for part in (slice(0, 300), slice(m - 300, m)):
+        want, z, _, scale = oracle.linear(x[part], w, b, "gelu", None)
+        oracle.close(y[part], want, 40 * E * scale + 16 * E * z.abs())
+
+
+def test_preference_over_a_corpus_past_32_bits(cvs):
+    rows = (1 << 31) // 1024 + 500
+    x = torch.zeros(rows, 1024, dtype=torch.float16, device="cuda")
+    x[:300] = randn(300, 1024, dtype=torch.float16, seed=1, scale=0.05)
+    x[-300:] = randn(300, 1024, dtype=torch.float16, seed=2, scale=0.05)
+    index = cvs.Index(x, metric="ip", copy=False)
+    q = randn(20, 1024, dtype=torch.float32, seed=3).requires_grad_()
+    c, rej = rows - 1 - ids(300, 20, seed=4), torch.cat([rows - 1 - ids(300, 20, 2, seed=5), ids(300, 20, 2, seed=6)], 1)
+    loss, m = index.preference_loss(q, c, rej, return_margins=True)
+    (dq,) = torch.autograd.grad(loss, q)
+    small = torch.cat([x[:300], x[-300:]])
+    there = cvs.Index(small, metric="ip")
+    near = lambda i: torch.where(i < 300, i, i - (rows - 600))  # noqa: E731
+    q2 = q.detach().requires_grad_()
+    loss2, m2 = there.preference_loss(q2, near(c), near(rej), return_margins=True)
+    (dq2,) = torch.autograd.grad(loss2, q2)
+    assert torch.equal(loss, loss2) and torch.equal(m, m2) and torch.equal(dq, dq2)
