@@ -31,7 +31,8 @@ BUILD = HERE / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CU_SOURCES = ["cvs_tc_search.cu", "cvs_tc_pair.cu", "cvs_gemv.cu", "cvs_merge.cu", "cvs_ingest.cu", "cvs_capi.cu",
-              "cvs_norm.cu", "cvs_linear.cu", "cvs_preference.cu", "cvs_adapter_capi.cu"]
+              "cvs_norm.cu", "cvs_linear.cu", "cvs_gemm_none.cu", "cvs_gemm_relu.cu", "cvs_gemm_gelu.cu",
+              "cvs_gemm_silu.cu", "cvs_preference.cu", "cvs_adapter_capi.cu"]
 EXT_SOURCES = ["torch_ext.cpp", "torch_adapter.cpp"]
 LIB_NAME = "libcvs_b200.so"
 

@@ -325,6 +325,7 @@ cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_
   if (z && (!aligned16(z) || z_stride % 8 != 0 || z_stride < n))
     return fail(CVS_ERR_INVALID_ARGUMENT, "z must be 16-byte aligned with a row stride that is a multiple of 8 and at least n");
   if (residual && m > 1 && residual_stride < 0) return fail(CVS_ERR_INVALID_ARGUMENT, "negative row stride");
+  if (activation == CVS_ACT_NONE) z = nullptr;  // only an activation's derivative reads it
   DeviceInfo dev;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
@@ -393,7 +394,7 @@ cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_
   GemmArgs a{};
   GemmProblem& p = a.p[0];
   set_shape(&p, t, m, n, k, 1);
-  p.act = activation;
+  a.act = activation;
   p.out = y;
   p.ld_out = y_stride;
   p.vec_out = mappable(y, y_stride, n);

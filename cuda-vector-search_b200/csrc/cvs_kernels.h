@@ -238,7 +238,6 @@ struct GemmProblem {
   int splits, kblocks, kper;
   int m, n;
   int a_mn, b_mn;        // operand stored with K as its outer dimension
-  int act;
   void* out;
   long long ld_out;
   const void* bias;      // [n] or null
@@ -252,6 +251,7 @@ struct GemmProblem {
 // Only p[0] may have a residual or z.
 struct GemmArgs {
   GemmProblem p[2];
+  int act;               // of p[0]; kActNone where there are two
   int bf16;
   int* err;
 };
@@ -261,7 +261,11 @@ struct GemmArgs {
 struct GemmMaps {
   CUtensorMap a[2], b[2], out[2], z, residual;
 };
-// Tile shapes: cg CTAs (128 rows each) x bn columns.
+// Tile shapes: cg CTAs (128 rows each) x bn columns. One translation unit per activation.
+cudaError_t gemm_launch_none(int cg, int bn, const GemmMaps& maps, const GemmArgs& a, int ctas, cudaStream_t stream);
+cudaError_t gemm_launch_relu(int cg, int bn, const GemmMaps& maps, const GemmArgs& a, int ctas, cudaStream_t stream);
+cudaError_t gemm_launch_gelu(int cg, int bn, const GemmMaps& maps, const GemmArgs& a, int ctas, cudaStream_t stream);
+cudaError_t gemm_launch_silu(int cg, int bn, const GemmMaps& maps, const GemmArgs& a, int ctas, cudaStream_t stream);
 cudaError_t gemm_launch(int cg, int bn, const GemmMaps& maps, const GemmArgs& a, int ctas, cudaStream_t stream);
 
 // One product of few 128 x 64 tiles, its K slices shared by the 2, 4 or 8 CTAs of a
