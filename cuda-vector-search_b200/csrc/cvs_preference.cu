@@ -83,16 +83,35 @@ __device__ __forceinline__ void prefetch_row(const void* q, int dtype, long long
   for (int c = lane * 128; c < d * es; c += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
 }
 
-// A row's norm, not below 1e-12.
+// What a cosine query is multiplied with: inv + lo = 1 / max(|q|, 1e-12) to about twice
+// fp32's digits. A margin against a reference is a small difference of two unit vectors,
+// and a rounding of the factor, unlike one of an element, moves all of the vector one
+// way: lo is one Newton step's correction of inv, from the sum of squares itself.
+struct UnitScale {
+  float inv = 1.f, lo = 0.f;
+  bool clamped = false;
+};
 template <int CPL>
-__device__ __forceinline__ float clamped_norm(const Pair (&u)[CPL][4]) {
-  Pair ss = both(0.f);
+__device__ __forceinline__ UnitScale unit_scale(const Pair (&u)[CPL][4]) {
+  Pair sq = both(0.f), sq2 = both(0.f);
 #pragma unroll
   for (int j = 0; j < CPL; ++j) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ss = pair_fma(u[j][i], u[j][i], ss);
+    for (int i = 0; i < 4; i += 2) {
+      sq = pair_fma(u[j][i], u[j][i], sq);
+      sq2 = pair_fma(u[j][i + 1], u[j][i + 1], sq2);
+    }
   }
-  return fmaxf(sqrtf(warp_sum(pair_total(ss))), 1e-12f);
+  const float ss = warp_sum(pair_total(pair_add(sq, sq2)));
+  const float norm = sqrtf(ss);
+  UnitScale s;
+  s.clamped = norm <= 1e-12f;
+  s.inv = __fdiv_rn(1.f, fmaxf(norm, 1e-12f));
+  if (!s.clamped && norm < 1e18f) {  // (beyond, the sum of squares is near overflow)
+    const float p = ss * s.inv, rest = fmaf(ss, s.inv, -p);
+    s.lo = 0.5f * s.inv * (fmaf(-p, s.inv, 1.f) - rest * s.inv);
+  }
+  return s;
 }
 
 // Group j of a staged row (zeros behind the row, which only the last group can reach).
@@ -222,7 +241,7 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
     const long long q = first + round * step;
     const bool live = q < a.b;
     Pair g[CPL][4];
-    float norm = 1.f, inv = 1.f;
+    UnitScale unit;
 #pragma unroll
     for (int j = 0; j < CPL; ++j) {
 #pragma unroll
@@ -239,21 +258,21 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
       load_pairs<CPL>(a.q, a.q_dtype, q * a.q_stride, a.d, a.q_vec, lane, u);
       if (a.ref) load_pairs<CPL>(a.ref, a.ref_dtype, q * a.ref_stride, a.d, a.ref_vec, lane, g);
       if (a.cosine) {
-        norm = clamped_norm<CPL>(u);
-        inv = __fdiv_rn(1.f, norm);
+        unit = unit_scale<CPL>(u);
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) u[j][i] = pair_mul(u[j][i], both(inv));
+          for (int i = 0; i < 4; ++i) u[j][i] = pair_fma(u[j][i], both(unit.inv), pair_mul(u[j][i], both(unit.lo)));
         }
       }
       if (a.ref) {
-        const Pair less = both(a.cosine ? -__fdiv_rn(1.f, clamped_norm<CPL>(g)) : -1.f);
+        UnitScale r;
+        if (a.cosine) r = unit_scale<CPL>(g);
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            u[j][i] = pair_fma(g[j][i], less, u[j][i]);
+            u[j][i] = pair_fma(g[j][i], both(-r.inv), pair_fma(g[j][i], both(-r.lo), u[j][i]));
             g[j][i] = both(0.f);
           }
         }
@@ -385,16 +404,16 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
       for (int j = 0; j < CPL; ++j) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          u[j][i] = pair_mul(u[j][i], both(inv));
+          u[j][i] = pair_mul(u[j][i], both(unit.inv));
           dot = pair_fma(u[j][i], g[j][i], dot);
         }
       }
       const float along_all = warp_sum(pair_total(dot));
-      const float along = norm > 1e-12f ? along_all : 0.f;  // below the clamp the divisor is a constant
+      const float along = unit.clamped ? 0.f : along_all;  // below the clamp the divisor is a constant
 #pragma unroll
       for (int j = 0; j < CPL; ++j) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) g[j][i] = pair_mul(pair_fma(u[j][i], both(-along), g[j][i]), both(inv));
+        for (int i = 0; i < 4; ++i) g[j][i] = pair_mul(pair_fma(u[j][i], both(-along), g[j][i]), both(unit.inv));
       }
     }
 #pragma unroll
