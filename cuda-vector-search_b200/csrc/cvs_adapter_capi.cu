@@ -165,8 +165,8 @@ BackwardPlan plan_backward(int64_t m, int n, int k, int sms) {
   // Both products run in one launch, with one tile shape, dw's work items first; item
   // i goes to CTA (pair) i mod slots. dw's K dimension (the rows) is cut into as many
   // parts as give the shortest of the longest queues, in slices of 64 along K plus one
-  // an item; each part costs the writing and reading of its fp32 sums (about what the
-  // SMs' share of half a slice takes, at 16 floats a thread and tile).
+  // an item; parts also cost the writing and reading of their fp32 sums, about three
+  // slices' time a round of them.
   b.tile = pick_tile(std::max<int64_t>(m, n), k, sms);
   const int slots = b.tile.slots(sms);
   const int64_t tiles = ceil_div(n, 128 * b.tile.cg) * ceil_div(k, b.tile.bn);

@@ -10,9 +10,12 @@
 // the product -- bias, activation, residual, the rounding to the rows' type -- is
 // done on the accumulator before it leaves the SM.
 //
-// Bound: 2 m n k operations at the tensor cores' rate for batches of hundreds of
-// rows and more; the weights' bytes below that, where linear_small_kernel (up to
-// kLinearSmallRows rows) streams them once with CUDA cores.
+// Bound: 2 m n k operations at the tensor cores' rate for batches of thousands of rows;
+// below that latency and the weights' bytes, where split_kernel shares K among a cluster
+// and linear_small_kernel (one or two rows) streams the weights once with CUDA cores.
+// Measured: 131072 x 1536 -> 768 bf16 with bias 220 us (1.41 PF/s), with residual 232 us;
+// 16384 x 768 -> 1536 with bias 33 us, forward for training with GELU 44 us, backward 96
+// us; 256 x 768 -> 1536 GELU 7.1 us; one row 2.5 us.
 //
 // The pre-activation z is kept for the backward pass as fp16, also for bf16 rows:
 // the activations' derivatives are constant where fp16 ends (|z| > 65504), and
@@ -279,7 +282,8 @@ constexpr int kDzRows = 4;    // rows a thread has in flight
 
 // dz = dy act'(z) in the rows' type (dz null: nothing to write, no activation), and
 // the block's share of every column's sum, in fp32 from the unrounded dz. Bound by
-// HBM: each thread has kDzRows rows' loads in flight before it computes.
+// HBM: each thread has kDzRows rows' loads in flight before it computes. 16384 x 1536:
+// ReLU 24 us, GELU 29 us (150 MB: 23 us at HBM rate).
 template <int ACT>
 __global__ void __launch_bounds__(32 * kDzWarps) linear_dz_kernel(const LinearDzArgs a) {
   grid_dependency_wait();

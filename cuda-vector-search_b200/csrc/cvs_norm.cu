@@ -18,7 +18,9 @@
 // every thread keeps the sums of dw and db for the columns it owns while its warp walks
 // the rows, so the weights' gradients cost no traffic per row; the blocks' sums go to the
 // workspace and a second small kernel adds them in a fixed order, which makes the result
-// the same on every run.
+// the same on every run. Measured: 262144 x 768 fp16 forward 140 us (5.8 TB/s), backward
+// 204 us (5.9 TB/s); with rows loaded into registers 157 and 372 us. 16384 x 768 bf16: 14
+// and 23 us, of which about half is the kernels' start and end.
 #include "cvs_device.cuh"
 #include "cvs_elem.cuh"
 #include "cvs_kernels.h"
@@ -111,7 +113,7 @@ __host__ __device__ constexpr bool norm_ring() { return VEC && WARPS == 1; }
 
 // STAGED: weights in shared memory, for blocks that walk many rows; otherwise straight
 // from global memory, where the staging and its barrier would be a large part of the
-// work (256 rows of 768: 5.2 us staged, 4.3 us straight; 262144 rows: 137 and 185 us).
+// work (256 rows of 768: 5.2 us staged, 4.3 us straight; 262144 rows: 140 and 185 us).
 template <class T, bool VEC, int WARPS, int CPL, bool STAGED>
 __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int kRowThreads = 32 * WARPS;

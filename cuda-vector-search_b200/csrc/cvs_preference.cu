@@ -23,7 +23,9 @@
 // bytes in flight do not depend on registers: with rows loaded into registers one or two
 // ahead, 16384 queries x 4 rejected rows of 768 columns took 113 us at an occupancy of 8
 // to 16 warps an SM. A stage's copies are issued together, a lane each, and waited for
-// together, which keeps the arithmetic's share of the instructions up.
+// together, which keeps the arithmetic's share of the instructions up. That size takes 61
+// us now (202 MB of rows, queries and results: 31 us at HBM rate), held by instructions
+// and their latency at the two blocks an SM that the registers allow.
 //
 // One warp takes a query, or 2, 4 or 8 warps share its rejected rows when there
 // are too few queries to fill the GPU with one warp each; the shares are added
