@@ -6,6 +6,7 @@
 #include "torch_adapter.h"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -42,8 +43,14 @@ int code(const Tensor& t) {
 int64_t pad8(int64_t v) { return (v + 7) / 8 * 8; }
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : pad8(t.size(1)); }
 
+// An uninitialised tensor on the device of `like`, without a trip through the
+// dispatcher (a training pass makes up to eight; each trip costs most of a microsecond).
+Tensor fresh(at::IntArrayRef sizes, torch::ScalarType type, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
 Tensor bytes(size_t n, const Tensor& like) {
-  return torch::empty({static_cast<int64_t>(std::max<size_t>(n, 256))}, like.options().dtype(torch::kUInt8));
+  return fresh({static_cast<int64_t>(std::max<size_t>(n, 256))}, torch::kUInt8, like);
 }
 
 // A 2-D tensor whose rows are contiguous; rows may be any distance apart.
@@ -56,7 +63,7 @@ Tensor with_tiles(const Tensor& t) {
                   (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1)));
   if (ok) return t;
   const Tensor src = with_rows(t);
-  const Tensor out = torch::empty({t.size(0), pad8(t.size(1))}, t.options());
+  const Tensor out = fresh({t.size(0), pad8(t.size(1))}, t.scalar_type(), t);
   check(cvs_align_rows(src.data_ptr(), row_stride(src), code(src), src.size(0), static_cast<int>(src.size(1)), out.data_ptr(),
                        out.size(1), stream_of(src)),
         "linear");
@@ -96,6 +103,10 @@ void first_order_only() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "the adapter's operators have no second derivative (create_graph=True)");
 }
 
+// What a backward pass has to know besides its tensors, in one number: a small code
+// (the weights' type, the activation) and which inputs there were.
+constexpr int64_t kHasWeight = 1 << 8, kHasBias = 1 << 9, kHasResidual = 1 << 10;
+
 Tensor or_undefined(const OptTensor& t) { return given(t) ? *t : Tensor(); }
 
 // Number of rows of a tensor seen as [rows, width].
@@ -111,10 +122,10 @@ NormOut norm_forward(const Tensor& x_in, const Tensor& weight, const Tensor& bia
   const Tensor x = with_rows(x_in);
   const int64_t rows = x.size(0), d = x.size(1);
   NormOut out;
-  out.y = torch::empty({rows, d}, x.options());
+  out.y = fresh({rows, d}, x.scalar_type(), x);
   if (keep) {
-    out.mean = torch::empty({rows}, x.options().dtype(torch::kFloat));
-    out.rstd = torch::empty({rows}, x.options().dtype(torch::kFloat));
+    out.mean = fresh({rows}, torch::kFloat, x);
+    out.rstd = fresh({rows}, torch::kFloat, x);
   }
   const Tensor& any = weight.defined() ? weight : bias;
   const Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
@@ -132,9 +143,8 @@ class LayerNormFn : public torch::autograd::Function<LayerNormFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
     NormOut out = norm_forward(x, or_undefined(weight), or_undefined(bias), eps, true);
     ctx->save_for_backward({x, or_undefined(weight), out.mean, out.rstd});
-    ctx->saved_data["weight"] = given(weight);
-    ctx->saved_data["bias"] = given(bias);
-    ctx->saved_data["type"] = given(bias) ? code(*bias) : (given(weight) ? code(*weight) : code(x));
+    const int64_t type = given(bias) ? code(*bias) : (given(weight) ? code(*weight) : code(x));
+    ctx->saved_data["layer"] = type | (given(weight) ? kHasWeight : 0) | (given(bias) ? kHasBias : 0);
     return out.y;
   }
 
@@ -143,16 +153,17 @@ class LayerNormFn : public torch::autograd::Function<LayerNormFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor x = with_rows(saved[0]), dy = with_rows(grads[0]);
     const c10::cuda::CUDAGuard guard(x.device());
-    const bool has_w = ctx->saved_data["weight"].toBool(), has_b = ctx->saved_data["bias"].toBool();
-    const int type = static_cast<int>(ctx->saved_data["type"].toInt());
+    const int64_t layer = ctx->saved_data["layer"].toInt();
+    const bool has_w = layer & kHasWeight, has_b = layer & kHasBias;
+    const int type = static_cast<int>(layer & 0xff);
     const Tensor w = has_w ? saved[1].contiguous() : Tensor();
     const int64_t rows = x.size(0), d = x.size(1);
-    const auto wopt = type == CVS_F32 ? x.options().dtype(torch::kFloat) : x.options();
+    const auto wtype = type == CVS_F32 ? torch::kFloat : x.scalar_type();
     size_t edge = 1;
     Tensor dx, dw, db;
-    if (ctx->needs_input_grad(0)) dx = torch::empty({rows, d}, x.options());
-    if (has_w && ctx->needs_input_grad(edge++)) dw = torch::empty({d}, wopt);
-    if (has_b && ctx->needs_input_grad(edge++)) db = torch::empty({d}, wopt);
+    if (ctx->needs_input_grad(0)) dx = fresh({rows, d}, x.scalar_type(), x);
+    if (has_w && ctx->needs_input_grad(edge++)) dw = fresh({d}, wtype, x);
+    if (has_b && ctx->needs_input_grad(edge++)) db = fresh({d}, wtype, x);
     size_t need = 0;
     Tensor ws;
     if (dw.defined() || db.defined()) {
@@ -212,8 +223,8 @@ LinearOut linear_forward(const Tensor& x_in, const Tensor& w_in, const Tensor& b
   const Tensor bias = bias_in.defined() ? bias_in.contiguous() : bias_in;
   const Tensor residual = residual_in.defined() ? with_rows(residual_in) : residual_in;
   LinearOut out;
-  out.y = torch::empty({m, n}, x.options());
-  if (keep) out.z = torch::empty({m, pad8(n)}, x.options().dtype(torch::kHalf));
+  out.y = fresh({m, n}, x.scalar_type(), x);
+  if (keep) out.z = fresh({m, pad8(n)}, torch::kHalf, x);
   check(cvs_linear(x.data_ptr(), row_stride(x), w.data_ptr(), row_stride(w), bias.defined() ? bias.data_ptr() : nullptr,
                    residual.defined() ? residual.data_ptr() : nullptr, residual.defined() ? row_stride(residual) : 0,
                    activation, code(x), m, static_cast<int>(n), static_cast<int>(k), out.y.data_ptr(), n,
@@ -234,17 +245,16 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
     // Where the product read aligned copies, the backward pass reads them again instead
     // of making its own (more than CVS_LINEAR_SMALL_ROWS rows; else the inputs as they are).
     ctx->save_for_backward({out.x, out.w, out.z});
-    ctx->saved_data["activation"] = activation;
-    ctx->saved_data["bias"] = given(bias);
-    ctx->saved_data["residual"] = given(residual);
+    ctx->saved_data["layer"] = activation | (given(bias) ? kHasBias : 0) | (given(residual) ? kHasResidual : 0);
     return out.y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order_only();
     const auto saved = ctx->get_saved_variables();
-    const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
-    const int activation = static_cast<int>(ctx->saved_data["activation"].toInt());
+    const int64_t layer = ctx->saved_data["layer"].toInt();
+    const bool has_b = layer & kHasBias, has_r = layer & kHasResidual;
+    const int activation = static_cast<int>(layer & 0xff);
     const c10::cuda::CUDAGuard guard(saved[0].device());
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     size_t edge = 2;
@@ -253,9 +263,9 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
     const Tensor& z = saved[2];
     const int64_t m = saved[0].size(0), k = saved[0].size(1), n = saved[1].size(0);
     Tensor dx, dw, db;
-    if (need_x) dx = torch::empty({m, k}, saved[0].options());
-    if (need_w) dw = torch::empty({n, k}, saved[0].options());
-    if (need_b) db = torch::empty({n}, saved[0].options());
+    if (need_x) dx = fresh({m, k}, saved[0].scalar_type(), saved[0]);
+    if (need_w) dw = fresh({n, k}, saved[0].scalar_type(), saved[0]);
+    if (need_b) db = fresh({n}, saved[0].scalar_type(), saved[0]);
     if (need_x || need_w || need_b) {
       const Tensor dy = with_rows(grads[0]);
       const Tensor x = need_w ? with_tiles(saved[0]) : saved[0], w = need_x ? with_tiles(saved[1]) : saved[1];
@@ -321,12 +331,11 @@ PreferenceOut preference_forward(const Tensor& q_in, const Tensor& ref_in, const
   const Tensor q = with_rows(q_in), ref = ref_in.defined() ? with_rows(ref_in) : ref_in;
   const Tensor chosen = chosen_in.contiguous(), rejected = with_rows(rejected_in);
   const int64_t b = q.size(0), d = q.size(1), r = rejected.size(1);
-  const auto f32 = corpus.options().dtype(torch::kFloat);
   PreferenceOut out;
-  out.loss = torch::empty({}, f32);
-  out.weight = torch::empty({}, f32);
-  out.margins = torch::empty({b, r}, f32);
-  if (keep) out.grad = torch::empty({b, pad8(d)}, f32);
+  out.loss = fresh({}, torch::kFloat, corpus);
+  out.weight = fresh({}, torch::kFloat, corpus);
+  out.margins = fresh({b, r}, torch::kFloat, corpus);
+  if (keep) out.grad = fresh({b, pad8(d)}, torch::kFloat, corpus);
   size_t need = 0;
   check(cvs_preference_loss_workspace_size(b, static_cast<int>(r), &need), "preference_loss");
   const Tensor ws = bytes(need, corpus);
@@ -363,7 +372,7 @@ class PreferenceFn : public torch::autograd::Function<PreferenceFn> {
     const int64_t b = grad.size(0), d = ctx->saved_data["width"].toInt();
     const auto type = static_cast<torch::ScalarType>(ctx->saved_data["type"].toInt());
     const Tensor upstream = grads[0].to(torch::kFloat);
-    Tensor dq = torch::empty({b, d}, grad.options().dtype(type));
+    Tensor dq = fresh({b, d}, type, grad);
     check(cvs_preference_grad(grad.data_ptr<float>(), grad.size(1), b, static_cast<int>(d), saved[1].data_ptr<float>(),
                               upstream.data_ptr<float>(), code(dq), dq.data_ptr(), stream_of(grad)),
           "preference_loss");

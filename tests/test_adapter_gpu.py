@@ -755,3 +755,42 @@ def test_preference_over_a_corpus_past_32_bits(cvs):
     loss2, m2 = there.preference_loss(q2, near(c), near(rej), return_margins=True)
     (dq2,) = torch.autograd.grad(loss2, q2)
     assert torch.equal(loss, loss2) and torch.equal(m, m2) and torch.equal(dq, dq2)
+
+
+# ---- several at once ----------------------------------------------------------------
+def test_threads_on_streams_of_their_own(cvs):
+    """Two host threads train and search at the same time, each on its own stream: both
+    get what they get alone."""
+    import threading
+
+    index = make_index(cvs, 3000, 384, "cosine")
+    adapters = [trained(cvs, 384, torch.bfloat16, seed=s) for s in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def work(s, out):
+        a = adapters[s]
+        with torch.cuda.stream(streams[s]):
+            got = []
+            for i in range(8):
+                q = randn(60 + 97 * s, 384, dtype=torch.bfloat16, seed=100 * s + i).requires_grad_()
+                b = q.shape[0]
+                loss, m = index.preference_loss(a(q), ids(3000, b, seed=i), ids(3000, b, 3, seed=i + 50), reference=q,
+                                                return_margins=True)
+                got.append((loss.detach(), m, *torch.autograd.grad(loss, (q, *a.parameters())),
+                            *index.search(q.detach(), 5, adapter=a)))
+            streams[s].synchronize()
+            out[s] = got
+
+    alone, together = {}, {}
+    for s in range(2):
+        work(s, alone)
+    threads = [threading.Thread(target=work, args=(s, together)) for s in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert sorted(together) == [0, 1]
+    for s in range(2):
+        for w, g in zip(alone[s], together[s]):
+            assert all(torch.equal(x, y) for x, y in zip(w, g))
