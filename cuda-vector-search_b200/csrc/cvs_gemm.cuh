@@ -304,12 +304,12 @@ __device__ __noinline__ void buf_to_rows(const uint8_t* buf, void* dst, long lon
 }
 __device__ __noinline__ void rows_to_buf(uint8_t* buf, const void* src, long long ld, int row0, int rows, int col0,
                                             int cols, int lane) {
-  // Eight rows' loads are under way before the first of them is staged.
+  // Sixteen rows' loads are under way before the first of them is staged.
 #pragma unroll
-  for (int r0 = 0; r0 < 32; r0 += 8) {
-    uint16_t v[8][2];
+  for (int r0 = 0; r0 < 32; r0 += 16) {
+    uint16_t v[16][2];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < 16; ++r) {
       const uint16_t* p = static_cast<const uint16_t*>(src) + (row0 + r0 + r) * ld + col0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -318,7 +318,7 @@ __device__ __noinline__ void rows_to_buf(uint8_t* buf, const void* src, long lon
       }
     }
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < 16; ++r) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int c = lane + 32 * h;

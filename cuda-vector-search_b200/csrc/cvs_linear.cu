@@ -284,51 +284,72 @@ constexpr int kDzRows = 4;    // rows a thread has in flight
 // the block's share of every column's sum, in fp32 from the unrounded dz. Bound by
 // HBM: each thread has kDzRows rows' loads in flight before it computes. 16384 x 1536:
 // ReLU 24 us, GELU 29 us (150 MB: 23 us at HBM rate).
-template <int ACT>
+// VEC: dy's rows are 16-byte aligned. Others come in two-byte loads that are consecutive
+// over the warp and are regrouped in shared memory (97742 x 339: 111 us with each lane
+// loading its own eight columns).
+template <int ACT, bool VEC>
 __global__ void __launch_bounds__(32 * kDzWarps) linear_dz_kernel(const LinearDzArgs a) {
   grid_dependency_wait();
   __shared__ float sums[kDzWarps][kDzCols];
+  __shared__ __align__(16) uint16_t rows_s[VEC ? 1 : kDzWarps][VEC ? 1 : kDzRows][VEC ? 8 : kDzCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = static_cast<int>(blockIdx.x) * kDzCols + lane * 8;
+  const int c0 = static_cast<int>(blockIdx.x) * kDzCols, c = c0 + lane * 8;
   const bool bf16 = a.bf16 != 0;
   float s[8];
 #pragma unroll
   for (int t = 0; t < 8; ++t) s[t] = 0.f;
-  if (c < a.n) {
-    const long long stride = static_cast<long long>(gridDim.y) * kDzWarps;
-    for (long long row0 = static_cast<long long>(blockIdx.y) * kDzWarps + warp; row0 < a.m; row0 += stride * kDzRows) {
-      uint4 g[kDzRows], z[kDzRows];
+  const long long stride = static_cast<long long>(gridDim.y) * kDzWarps;
+  for (long long row0 = static_cast<long long>(blockIdx.y) * kDzWarps + warp; row0 < a.m; row0 += stride * kDzRows) {
+    uint4 g[kDzRows], z[kDzRows];
+#pragma unroll
+    for (int i = 0; i < kDzRows; ++i) {
+      const long long row = row0 + i * stride;
+      g[i] = z[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (row >= a.m || c >= a.n) continue;
+      if constexpr (VEC) g[i] = load_unit8(static_cast<const uint16_t*>(a.dy) + row * a.ld_dy + c, c, a.n, true);
+      // z's rows are padded to whole units; what lies in the padding meets a dy of zero below.
+      if constexpr (ACT != kActNone)
+        z[i] = load_unit8(static_cast<const uint16_t*>(a.z) + row * a.ld_z + c, c, a.n, true);
+    }
+    if constexpr (!VEC) {
+      uint16_t v[kDzRows][8];
 #pragma unroll
       for (int i = 0; i < kDzRows; ++i) {
         const long long row = row0 + i * stride;
-        g[i] = z[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < a.m) {
-          g[i] = load_unit8(static_cast<const uint16_t*>(a.dy) + row * a.ld_dy + c, c, a.n, a.vec_dy != 0);
-          // z's rows are padded to whole units; what lies in the padding meets a dy of zero below.
-          if constexpr (ACT != kActNone)
-            z[i] = load_unit8(static_cast<const uint16_t*>(a.z) + row * a.ld_z + c, c, a.n, true);
-        }
+        const uint16_t* p = static_cast<const uint16_t*>(a.dy) + row * a.ld_dy + c0 + lane;
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          v[i][t] = row < a.m && c0 + 32 * t + lane < a.n ? p[32 * t] : static_cast<uint16_t>(0);
       }
 #pragma unroll
       for (int i = 0; i < kDzRows; ++i) {
-        const long long row = row0 + i * stride;
-        if (row >= a.m) continue;
-        const uint32_t gs[4] = {g[i].x, g[i].y, g[i].z, g[i].w}, zs[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
-        uint32_t o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float2 f = unpack2(gs[e], bf16);
-          if constexpr (ACT != kActNone) {
-            const float2 zf = unpack2(zs[e], false);
-            slope_pair<ACT>(zf.x, zf.y, f.x, f.y);
-          }
-          s[2 * e] += f.x;
-          s[2 * e + 1] += f.y;
-          o[e] = pack2(f.x, f.y, bf16);
-        }
-        if (a.dz)
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dz) + row * a.ld_dz + c) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int t = 0; t < 8; ++t) rows_s[warp][i][32 * t + lane] = v[i][t];
       }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kDzRows; ++i) g[i] = *reinterpret_cast<const uint4*>(&rows_s[warp][i][lane * 8]);
+      __syncwarp();
+    }
+#pragma unroll
+    for (int i = 0; i < kDzRows; ++i) {
+      const long long row = row0 + i * stride;
+      if (row >= a.m || c >= a.n) continue;
+      const uint32_t gs[4] = {g[i].x, g[i].y, g[i].z, g[i].w}, zs[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
+      uint32_t o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float2 f = unpack2(gs[e], bf16);
+        if constexpr (ACT != kActNone) {
+          const float2 zf = unpack2(zs[e], false);
+          slope_pair<ACT>(zf.x, zf.y, f.x, f.y);
+        }
+        s[2 * e] += f.x;
+        s[2 * e + 1] += f.y;
+        o[e] = pack2(f.x, f.y, bf16);
+      }
+      if (a.dz)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dz) + row * a.ld_dz + c) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
   grid_launch_dependents();
@@ -521,14 +542,22 @@ int linear_dz_parts(long long m, int n, int num_sms) {
   return static_cast<int>(std::max<long long>(1, std::min<long long>(want, (m + kDzWarps - 1) / kDzWarps)));
 }
 
+namespace {
+template <int ACT>
+cudaError_t dz_launch_act(const LinearDzArgs& a, dim3 grid, cudaStream_t stream) {
+  const dim3 block(32 * kDzWarps);
+  return a.vec_dy ? launch_programmatic(linear_dz_kernel<ACT, true>, grid, block, 0, stream, a)
+                  : launch_programmatic(linear_dz_kernel<ACT, false>, grid, block, 0, stream, a);
+}
+}  // namespace
+
 cudaError_t linear_dz_launch(const LinearDzArgs& a, int parts, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>((a.n + kDzCols - 1) / kDzCols), static_cast<unsigned>(parts));
-  const dim3 block(32 * kDzWarps);
   switch (a.z ? a.act : kActNone) {
-    case kActNone: return launch_programmatic(linear_dz_kernel<kActNone>, grid, block, 0, stream, a);
-    case kActRelu: return launch_programmatic(linear_dz_kernel<kActRelu>, grid, block, 0, stream, a);
-    case kActGelu: return launch_programmatic(linear_dz_kernel<kActGelu>, grid, block, 0, stream, a);
-    case kActSilu: return launch_programmatic(linear_dz_kernel<kActSilu>, grid, block, 0, stream, a);
+    case kActNone: return dz_launch_act<kActNone>(a, grid, stream);
+    case kActRelu: return dz_launch_act<kActRelu>(a, grid, stream);
+    case kActGelu: return dz_launch_act<kActGelu>(a, grid, stream);
+    case kActSilu: return dz_launch_act<kActSilu>(a, grid, stream);
     default: return cudaErrorInvalidValue;
   }
 }
