@@ -272,11 +272,15 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
   return r;
 }
 
-// Every thread of both CTAs of the cluster arrives and waits.
+// Every thread of every CTA of the cluster arrives; a thread that then waits knows that
+// all of them have.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Every thread of every CTA of the cluster arrives and waits.
 __device__ __forceinline__ void cluster_sync_all() {
-  asm volatile(
-      "barrier.cluster.arrive.release.aligned;\n\t"
-      "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 
 // Shared::cluster address of the same shared variable in CTA `rank`.

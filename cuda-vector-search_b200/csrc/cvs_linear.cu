@@ -35,7 +35,9 @@ namespace {
 // dimension. Each sends its fp32 sums of column slice c to CTA c through distributed
 // shared memory; after one cluster barrier CTA c adds the S parts in order and finishes
 // its 64 / S columns (bias, activation, residual). No workspace, one launch, the same
-// result every run.
+// result every run. Another CTA's shared memory exists only once that CTA has started:
+// every thread arrives on a cluster barrier in the prologue and waits for it after the
+// products, ahead of the first store to a peer.
 constexpr int kSplitN = 64;
 constexpr int kSplitStages = 3;
 constexpr int kSplitThreads = 192;
@@ -83,6 +85,7 @@ __global__ void __launch_bounds__(kSplitThreads)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  cluster_arrive();
   const uint32_t tmem = *tmem_holder;
   grid_dependency_wait();
   if (warp == 0) {
@@ -103,6 +106,7 @@ __global__ void __launch_bounds__(kSplitThreads)
       }
     }
     __syncwarp();
+    cluster_wait();
   } else if (warp == 1) {
     if (elect_one_lane()) {
       const uint32_t idesc = gemm_idesc(kGemmM, kSplitN, a.bf16 != 0, false, false);
@@ -121,11 +125,14 @@ __global__ void __launch_bounds__(kSplitThreads)
       mbar_wait_drain(done, 0);
     }
     __syncwarp();
+    cluster_wait();
   } else {
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
     const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, abort, a.err, 46));
     tc_fence_after();
+    __syncwarp();
+    cluster_wait();  // every CTA of the cluster has started
     const uint32_t parts = smem_u32(base + L::kParts);
     constexpr int kQ = kSplitN / S / 4;  // float4 groups per slice
 #pragma unroll
