@@ -120,6 +120,9 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const __grid
   constexpr int kRowsPerBlock = kNormThreads / kRowThreads;
   constexpr bool kRing = STAGED && norm_ring<VEC, WARPS>();
   constexpr int kRows = WARPS == 1 && !kRing ? kForwardRows : 1;  // rows a warp (block) has at work
+  // The first group of columns that a row may end in (launch_width: every width of one warp
+  // has its own CPL; a block's has 1, 2 or 4, and the row fills more than half of them).
+  constexpr int kFirstPartial = WARPS == 1 ? CPL - 1 : CPL / 2;
   __shared__ float2 scratch[2][WARPS > 1 ? WARPS : 1];
   __shared__ __align__(8) uint64_t bars[kRing ? kNormWarps : 1][kRing ? kForwardSlots : 1];
   __shared__ int abort_s;
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           Pair c = pair_add(pair_at(raw[q][j], i), shift);
-          if (!VEC || j == CPL - 1) c = inside<VEC>(c, d, tid, kRowThreads, j, i);
+          if (!VEC || j >= kFirstPartial) c = inside<VEC>(c, d, tid, kRowThreads, j, i);
           sq = pair_fma(c, c, sq);
         }
       }

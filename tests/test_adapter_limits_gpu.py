@@ -4,9 +4,19 @@ import pytest
 import torch
 
 import adapter_oracle as oracle
-from test_adapter_gpu import E, cvs, randn  # noqa: F401  (cvs: the fixture)
+from test_adapter_gpu import DTYPES, E, check_norm, cvs, randn  # noqa: F401  (cvs: the fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- layer norm -------------------------------------------------------------------
+# One block of 256 threads takes a row wider than 4096 in four groups of 2048 columns.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [4104, 5120, 6136, 6144, 6152, 7000])
+def test_layer_norm_widths_that_end_before_the_last_group(cvs, dtype, d):
+    t = DTYPES[dtype]
+    check_norm(cvs, randn(9, d, dtype=t, seed=1, shift=3.0), randn(d, dtype=t, seed=2, shift=1.0), randn(d, dtype=t, seed=3),
+               randn(9, d, dtype=t, seed=4))
 
 
 # ---- few tiles: K shared by a cluster ---------------------------------------------------
