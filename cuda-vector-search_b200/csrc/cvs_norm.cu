@@ -490,12 +490,12 @@ cudaError_t launch_one(NormArgs a, bool backward, int num_sms, cudaStream_t stre
         const size_t per = static_cast<size_t>(kNormWarps) * a.d * sizeof(T);
         a.slots = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kForwardSlots, (72 * 1024 - smem) / per)));
         smem += a.slots * per;
-        if (smem > 32 * 1024) {
-          const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-          if (e != cudaSuccess) return e;
-        }
       } else if (WARPS == 1) {
         per_warp = kForwardRows;
+      }
+      if (smem > 32 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
       }
       const unsigned grid = norm_grid(a.rows, kPerBlock * per_warp, blocks_per_sm(kern, smem) * num_sms);
       return launch_programmatic(kern, dim3(grid), dim3(kNormThreads), smem, stream, a);

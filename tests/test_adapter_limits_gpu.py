@@ -19,6 +19,14 @@ def test_layer_norm_widths_that_end_before_the_last_group(cvs, dtype, d):
                randn(9, d, dtype=t, seed=4))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,d", [(2048, 4104), (2500, 8191), (2500, 8192)])
+def test_layer_norm_many_wide_rows(cvs, dtype, rows, d):
+    t = DTYPES[dtype]
+    check_norm(cvs, randn(rows, d, dtype=t, seed=1, shift=0.5), randn(d, dtype=t, seed=2, shift=1.0),
+               randn(d, dtype=t, seed=3), randn(rows, d, dtype=t, seed=4))
+
+
 # ---- few tiles: K shared by a cluster ---------------------------------------------------
 @pytest.mark.parametrize("m,k", [(3, 384), (100, 384), (3, 576), (100, 576)])
 def test_linear_clusters_with_ctas_without_a_slice(cvs, m, k):
