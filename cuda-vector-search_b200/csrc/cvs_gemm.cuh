@@ -713,19 +713,6 @@ __global__ void __launch_bounds__(GemmShape<CG, BN>::kThreads, 1)
   }
 }
 
-// Sets a kernel's dynamic shared memory limit, once per device.
-template <class K>
-cudaError_t allow_smem(K kern, int smem, std::atomic<unsigned long long>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
-  return e;
-}
-
 template <int CG, int BN, int ACT, bool RES, bool Z>
 cudaError_t gemm_launch_one(const GemmMaps& maps, const GemmArgs& a, int ctas, cudaStream_t stream) {
   using S = GemmShape<CG, BN>;

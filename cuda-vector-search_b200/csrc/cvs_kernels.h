@@ -6,6 +6,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
@@ -169,6 +170,21 @@ cudaError_t launch_programmatic(void (*kernel)(Params...), dim3 grid, dim3 block
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Args&&>(args)...);
+}
+
+// Sets a kernel's dynamic shared memory limit, once per device. The limit belongs to the
+// kernel, not to a launch, so `smem` is the most that any call of it asks for: one that
+// followed the call's own size could be lowered by another thread before the launch.
+template <class K>
+cudaError_t allow_smem(K kern, int smem, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 struct MergeListsArgs {

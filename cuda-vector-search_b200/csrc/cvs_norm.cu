@@ -37,6 +37,7 @@ constexpr int kNormWarps = kNormThreads / 32;
 constexpr int kNormSlots = 4;    // most row pairs in a warp's ring of the backward pass
 constexpr int kForwardSlots = 8; // most rows in a warp's ring of the forward pass
 constexpr int kForwardRows = 2;  // rows a warp has at work in the forward pass
+constexpr int kForwardShared = 72 * 1024;  // most shared memory of a staged forward block: weight and bias, the ring
 
 // Sum over the threads of a row: one warp, or all 8 warps of the block (scratch
 // holds two buffers used in turn, so one barrier per sum is enough).
@@ -263,8 +264,11 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const __grid
 // registers, which the sums of dw and db need (16 a group of columns); other rows are
 // loaded into registers, the next row's loads under way where that fits. Two blocks an
 // SM, except for wide fp32 rows.
+template <class T, int CPL>
+constexpr int backward_blocks() { return sizeof(T) == 4 && CPL > 3 ? 1 : 2; }
+
 template <class T, bool VEC, int WARPS, int CPL>
-__global__ void __launch_bounds__(kNormThreads, sizeof(T) == 4 && CPL > 3 ? 1 : 2)
+__global__ void __launch_bounds__(kNormThreads, (backward_blocks<T, CPL>()))
     norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int kRowThreads = 32 * WARPS;
   constexpr int kRowsPerBlock = kNormThreads / kRowThreads;
@@ -488,36 +492,35 @@ cudaError_t launch_one(NormArgs a, bool backward, int num_sms, cudaStream_t stre
       int per_warp = 1;  // rows a warp has at work
       if (norm_ring<VEC, WARPS>()) {
         const size_t per = static_cast<size_t>(kNormWarps) * a.d * sizeof(T);
-        a.slots = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kForwardSlots, (72 * 1024 - smem) / per)));
+        a.slots = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kForwardSlots, (kForwardShared - smem) / per)));
         smem += a.slots * per;
       } else if (WARPS == 1) {
         per_warp = kForwardRows;
       }
-      if (smem > 32 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
-      }
+      static std::atomic<unsigned long long> allowed{0};
+      const cudaError_t e = allow_smem(kern, kForwardShared, allowed);
+      if (e != cudaSuccess) return e;
       const unsigned grid = norm_grid(a.rows, kPerBlock * per_warp, blocks_per_sm(kern, smem) * num_sms);
       return launch_programmatic(kern, dim3(grid), dim3(kNormThreads), smem, stream, a);
     }
     const unsigned grid = norm_grid(a.rows, WARPS == 1 ? kPerBlock * kForwardRows : 1, INT_MAX);
     return launch_programmatic(norm_forward_kernel<T, VEC, WARPS, CPL, false>, dim3(grid), dim3(kNormThreads), 0, stream, a);
   }
+  constexpr int kShared = backward_blocks<T, CPL>() == 1 ? 216 * 1024 : 108 * 1024;  // most of any call
   const size_t sums = WARPS == 1 && a.partial ? static_cast<size_t>(kNormWarps) * 2 * a.d * 4 : 0;
   size_t ring = 0;
   a.slots = 1;
   if (norm_ring<VEC, WARPS>()) {
     const size_t per = static_cast<size_t>(kNormWarps) * 2 * a.d * sizeof(T);
-    const size_t room = (sizeof(T) == 4 && CPL > 3 ? 216 : 108) * 1024 - weights;
+    const size_t room = kShared - weights;
     a.slots = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kNormSlots, room / per)));
     ring = a.slots * per;
   }
   const size_t smem = std::max(weights + ring, sums);
   auto kern = norm_backward_kernel<T, VEC, WARPS, CPL>;
-  if (smem > 32 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-  }
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_smem(kern, kShared, allowed);
+  if (e != cudaSuccess) return e;
   const unsigned grid = static_cast<unsigned>(norm_backward_blocks(a.rows, a.d, num_sms));
   return launch_programmatic(kern, dim3(grid), dim3(kNormThreads), smem, stream, a);
 }

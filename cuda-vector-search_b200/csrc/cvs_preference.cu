@@ -507,17 +507,19 @@ int pref_warps(long long b, int r, int num_sms) {
   return w;
 }
 
-// Rows of a stage: two blocks an SM up to 1024 columns, one block beyond.
-int pref_stage_rows(int d_pad, size_t shares) {
+// Shared memory of a block: two blocks an SM up to 1024 columns, one block beyond.
+constexpr int pref_shared(int cpl) { return cpl <= 4 ? 108 * 1024 : 216 * 1024; }
+
+// Rows of a stage.
+int pref_stage_rows(int d_pad, int cpl, size_t shares) {
   const size_t per = static_cast<size_t>(2 * kPrefWarps) * d_pad * 2;
-  const size_t room = d_pad <= 1024 ? 108 * 1024 : 216 * 1024;
-  return static_cast<int>(std::max<size_t>(1, std::min<size_t>(kPrefStageRows, (room - shares) / per)));
+  return static_cast<int>(std::max<size_t>(1, std::min<size_t>(kPrefStageRows, (pref_shared(cpl) - shares) / per)));
 }
 
 template <int CPL>
 cudaError_t pref_launch_one(const PreferenceArgs& a, unsigned grid, size_t smem, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(preference_kernel<CPL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_smem(preference_kernel<CPL>, pref_shared(CPL), allowed);
   if (e != cudaSuccess) return e;
   return launch_programmatic(preference_kernel<CPL>, dim3(grid), dim3(kPrefThreads), smem, stream, a);
 }
@@ -533,9 +535,9 @@ cudaError_t preference_launch(PreferenceArgs a, int mean, float* loss, float* we
   a.warps_per_query = pref_warps(a.b, a.r, num_sms);
   const unsigned grid = static_cast<unsigned>(preference_blocks(a.b, a.r, num_sms));
   const size_t shares = a.grad && a.warps_per_query > 1 ? static_cast<size_t>(kPrefWarps) * a.d_pad * 4 : 0;
-  a.stage_rows = pref_stage_rows(a.d_pad, shares);
-  const size_t smem = static_cast<size_t>(2 * kPrefWarps) * a.stage_rows * a.d_pad * 2 + shares;
   const int cpl = (a.d_pad / 8 + 31) / 32;
+  a.stage_rows = pref_stage_rows(a.d_pad, cpl, shares);
+  const size_t smem = static_cast<size_t>(2 * kPrefWarps) * a.stage_rows * a.d_pad * 2 + shares;
   cudaError_t e;
   if (a.b == 0) {
     e = cudaSuccess;

@@ -1,12 +1,29 @@
 """The adapter's operators where a first set of sizes did not look."""
 
+import ctypes
+import threading
+from pathlib import Path
+
 import pytest
 import torch
 
 import adapter_oracle as oracle
-from test_adapter_gpu import DTYPES, E, check_norm, cvs, randn  # noqa: F401  (cvs: the fixture)
+from test_adapter_gpu import DTYPES, E, check_norm, cvs, ids, randn  # noqa: F401  (cvs: the fixture)
 
 pytestmark = pytest.mark.gpu
+
+LIB = Path(__file__).resolve().parent.parent / "cuda-vector-search_b200" / "cuda_vector_search" / "libcvs_b200.so"
+vp, i64, i32, f32, size = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+
+
+@pytest.fixture(scope="module")
+def lib():
+    lib = ctypes.CDLL(str(LIB))
+    lib.cvs_last_error.restype = ctypes.c_char_p
+    lib.cvs_layer_norm.argtypes = [vp, i32, i64, i32, i64, vp, vp, i32, f32, vp, i64, vp, vp, vp]
+    lib.cvs_preference_loss.argtypes = [vp, i32, i64, vp, i32, i64, i64, i32, i32, vp, i64, i32, vp, vp, i64, i32, f32, f32,
+                                        i32, vp, vp, vp, vp, i64, vp, size, vp]
+    return lib
 
 
 # ---- layer norm -------------------------------------------------------------------
@@ -39,3 +56,74 @@ def test_linear_clusters_with_ctas_without_a_slice(cvs, m, k):
     first = cvs.linear(x, w)
     oracle.close(first, want, (k / 8 + 16) * E * scale)
     assert all(torch.equal(cvs.linear(x, w), first) for _ in range(200))
+
+
+# ---- two host threads ---------------------------------------------------------------
+def in_threads(*calls, repeats=4000):
+    """Each call over and over in a host thread of its own (foreign calls release the
+    interpreter lock); the first error of each."""
+    errors = [None] * len(calls)
+    start = threading.Barrier(len(calls))
+
+    def work(j):
+        start.wait()
+        for _ in range(repeats):
+            why = calls[j]()
+            if why:
+                errors[j] = why
+                return
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return errors
+
+
+def test_layer_norm_of_two_widths_from_two_threads(lib):
+    """Both widths run the same kernel with different amounts of shared memory."""
+    rows, out, calls = 16384, [], []
+    for j, d in enumerate((520, 768)):
+        x = randn(rows, d, dtype=torch.float16, seed=j)
+        y = torch.empty_like(x)
+        s = torch.cuda.Stream()
+
+        def call(x=x, y=y, d=d, s=s):
+            st = lib.cvs_layer_norm(x.data_ptr(), 1, rows, d, d, None, None, 1, 1e-5, y.data_ptr(), d, None, None, s.cuda_stream)
+            return lib.cvs_last_error() if st else None
+
+        calls.append(call)
+        out.append((x, y))
+    torch.cuda.synchronize()
+    assert in_threads(*calls) == [None, None]
+    for x, y in out:
+        want = oracle.layer_norm(x, None, None, 1e-5)
+        oracle.close(y, want, 200 * E * (1 + want.abs()))
+
+
+def test_preference_loss_of_two_widths_from_two_threads(lib):
+    b, r, n, keep, calls = 64, 2, 200, [], []
+    for j, d in enumerate((64, 256)):
+        q = randn(b, d, dtype=torch.float32, seed=j)
+        x = randn(n, d, dtype=torch.float16, seed=5 + j)
+        chosen, rejected = ids(n, b, seed=7), ids(n, b, r, seed=8)
+        loss, weight = torch.empty(1, device="cuda"), torch.empty(1, device="cuda")
+        margins, ws = torch.empty(b, r, device="cuda"), torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
+        s = torch.cuda.Stream()
+
+        def call(q=q, x=x, d=d, chosen=chosen, rejected=rejected, loss=loss, weight=weight, margins=margins, ws=ws, s=s):
+            st = lib.cvs_preference_loss(q.data_ptr(), 0, d, None, 0, 0, b, d, 0, x.data_ptr(), n, d, chosen.data_ptr(),
+                                         rejected.data_ptr(), r, r, 1.0, 0.0, 1, loss.data_ptr(), weight.data_ptr(),
+                                         margins.data_ptr(), None, 0, ws.data_ptr(), ws.numel(), s.cuda_stream)
+            return lib.cvs_last_error() if st else None
+
+        calls.append(call)
+        keep.append((q, x, chosen, rejected, margins))
+    torch.cuda.synchronize()
+    assert in_threads(*calls) == [None, None]
+    for q, x, chosen, rejected, margins in keep:
+        _, want, _ = oracle.preference(q, None, chosen, rejected, x, False, 1.0, 0.0, True)
+        sizes = x.double().abs()[chosen][:, None] + x.double().abs()[rejected]
+        oracle.close(margins, want, 150 * E * (sizes * q.double().abs()[:, None]).sum(2))
