@@ -28,6 +28,20 @@ cvs_status check_workspace(const void* ws, size_t have, size_t need) {
 }
 
 // ---- layer norm -----------------------------------------------------------------
+thread_local int64_t g_norm_stall = 0;  // armed failure-path test (cvs_debug_stall_next_norm)
+
+// Launches, with the device error word that the kernels' bounded waits report to.
+cvs_status run_norm(NormArgs& a, int dtype, bool backward, const DeviceInfo& dev, cudaStream_t s) {
+  a.err = dev.err;
+  a.wait_cycles = g_norm_stall;
+  a.stall = g_norm_stall > 0;
+  g_norm_stall = 0;  // one call only
+  const cudaError_t e = norm_launch(a, dtype, backward, dev.sms, s);
+  if (a.stall && e == cudaErrorNotSupported)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "the stall test hook needs aligned rows of up to 1024 columns (forward: 16384 of them)");
+  return e == cudaSuccess ? CVS_OK : cuda_fail(e, backward ? "layer norm backward launch" : "layer norm launch");
+}
+
 cvs_status check_norm(int dtype, int64_t rows, int d, int64_t x_stride, int weight_dtype) {
   if (rows < 0) return fail(CVS_ERR_INVALID_ARGUMENT, "row count must be >= 0");
   if (d < 1 || d > CVS_MAX_NORM_WIDTH)
@@ -238,8 +252,7 @@ cvs_status cvs_layer_norm(const void* x, int dtype, int64_t rows, int d, int64_t
   a.y_stride = y_stride;
   a.mean = mean;
   a.rstd = rstd;
-  const cudaError_t e = norm_launch(a, dtype, false, dev.sms, static_cast<cudaStream_t>(stream));
-  return e == cudaSuccess ? CVS_OK : cuda_fail(e, "layer norm launch");
+  return run_norm(a, dtype, false, dev, static_cast<cudaStream_t>(stream));
 }
 
 cvs_status cvs_layer_norm_backward_workspace_size(int64_t rows, int d, size_t* bytes) {
@@ -295,9 +308,14 @@ cvs_status cvs_layer_norm_backward(const void* dy, int64_t dy_stride, const void
   a.dweight = dweight;
   a.dbias = dbias;
   a.partial = sums ? static_cast<float*>(workspace) : nullptr;
-  a.err = dev.err;
-  const cudaError_t e = norm_launch(a, dtype, true, dev.sms, s);
-  return e == cudaSuccess ? CVS_OK : cuda_fail(e, "layer norm backward launch");
+  return run_norm(a, dtype, true, dev, s);
+}
+
+cvs_status cvs_debug_stall_next_norm(int64_t wait_cycles) {
+  if (wait_cycles < 1000 || wait_cycles > (int64_t{1} << 40))
+    return fail(CVS_ERR_INVALID_ARGUMENT, "wait_cycles must be in 1000 .. 2^40 (got %lld)", (long long)wait_cycles);
+  g_norm_stall = wait_cycles;
+  return CVS_OK;
 }
 
 cvs_status cvs_align_rows(const void* src, int64_t src_stride, int dtype, int64_t rows, int cols, void* dst,

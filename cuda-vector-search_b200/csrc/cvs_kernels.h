@@ -234,8 +234,12 @@ struct NormArgs {
   void* dweight;       // null: not wanted
   void* dbias;
   float* partial;      // [blocks][2][d] or null when neither dweight nor dbias is wanted
-  int* err;
+  int* err;            // device error word (the rings' waits are bounded)
   int slots;           // set by norm_launch: row pairs in a warp's ring
+  // Failure-path test hook (kernels with a ring; cvs_debug_stall_next_norm): stall != 0
+  // copies no row, and wait_cycles > 0 replaces the waits' usual limit.
+  int stall;
+  long long wait_cycles;
 };
 // Blocks of the backward kernel, each with its own row of `partial`.
 int norm_backward_blocks(long long rows, int d, int num_sms);

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const __grid
   const uint32_t row_bytes = static_cast<uint32_t>(d) * sizeof(T);
   uint8_t* ring = shared_f + 2 * CPL * 4 * kRowThreads * sizeof(float2) + static_cast<size_t>(warp) * a.slots * row_bytes;
   const auto request = [&](long long r, int k) {  // one lane
-    if (r >= a.rows) return;
+    if (r >= a.rows || a.stall) return;
     mbar_arrive_expect_tx(&bars[warp][k], row_bytes);
     bulk_load(ring + k * row_bytes, static_cast<const T*>(a.x) + r * a.x_stride, row_bytes, &bars[warp][k]);
   };
@@ -165,11 +165,12 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const __grid
   int slot = 0;
   uint32_t parity = 0;
   bool ok = true;
+  const long long limit = a.wait_cycles > 0 ? a.wait_cycles : kWaitCycles;
   for (; row0 < a.rows; row0 += slots * kRows) {
     Raw8<T> raw[kRows][CPL];
     float mean[kRows], rstd[kRows];
     if constexpr (kRing) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][slot], parity, &abort_s, a.err, 42));
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][slot], parity, &abort_s, a.err, 42, limit));
       if (!ok) break;
     }
 #pragma unroll
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const __grid
     }
   }
   if constexpr (kRing) {
-    if (!ok && lane == 0) {  // after a wait that ran out: copies under way land
+    if (!ok && !a.stall && lane == 0) {  // after a wait that ran out: copies under way land
       for (int k = 0; k < a.slots; ++k, row0 += slots) {
         if (row0 < a.rows) mbar_wait_drain(&bars[warp][(slot + k) % a.slots], slot + k < a.slots ? parity : parity ^ 1);
       }
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(kNormThreads, (backward_blocks<T, CPL>()))
   const uint32_t row_bytes = static_cast<uint32_t>(d) * sizeof(T);
   uint8_t* ring = shared_b + CPL * 4 * kRowThreads * sizeof(float2) + static_cast<size_t>(warp) * a.slots * 2 * row_bytes;
   const auto request = [&](long long r, int k) {  // one lane
-    if (r >= a.rows) return;
+    if (r >= a.rows || a.stall) return;
     mbar_arrive_expect_tx(&bars[warp][k], 2 * row_bytes);
     bulk_load(ring + k * 2 * row_bytes, static_cast<const T*>(a.x) + r * a.x_stride, row_bytes, &bars[warp][k]);
     bulk_load(ring + k * 2 * row_bytes + row_bytes, static_cast<const T*>(a.dy) + r * a.dy_stride, row_bytes, &bars[warp][k]);
@@ -323,6 +324,7 @@ __global__ void __launch_bounds__(kNormThreads, (backward_blocks<T, CPL>()))
   int turn = 0, slot = 0;
   uint32_t parity = 0;
   bool ok = true;
+  const long long limit = a.wait_cycles > 0 ? a.wait_cycles : kWaitCycles;
   for (; row < a.rows; row += slots, turn ^= 1) {
     const float mean = mean_n, rstd = rstd_n;
     if (row + slots < a.rows) {
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kNormThreads, (backward_blocks<T, CPL>()))
     }
     const T *xs, *gs;  // this row
     if constexpr (kRing) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][slot], parity, &abort_s, a.err, 41));
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][slot], parity, &abort_s, a.err, 41, limit));
       if (!ok) break;
       xs = reinterpret_cast<const T*>(ring + slot * 2 * row_bytes);
       gs = reinterpret_cast<const T*>(ring + slot * 2 * row_bytes + row_bytes);
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(kNormThreads, (backward_blocks<T, CPL>()))
     }
   }
   if constexpr (kRing) {
-    if (!ok && lane == 0) {  // after a wait that ran out: copies under way land
+    if (!ok && !a.stall && lane == 0) {  // after a wait that ran out: copies under way land
       for (int k = 0; k < a.slots; ++k, row += slots) {
         if (row < a.rows) mbar_wait_drain(&bars[warp][(slot + k) % a.slots], slot + k < a.slots ? parity : parity ^ 1);
       }
@@ -484,6 +486,7 @@ template <class T, bool VEC, int WARPS, int CPL>
 cudaError_t launch_one(NormArgs a, bool backward, int num_sms, cudaStream_t stream) {
   constexpr int kPerBlock = kNormWarps / WARPS;
   const size_t weights = static_cast<size_t>(CPL) * 4 * 32 * WARPS * sizeof(float2);
+  if (a.stall && !(norm_ring<VEC, WARPS>() && (backward || norm_staged(a.rows, a.d)))) return cudaErrorNotSupported;
   if (!backward) {
     if (norm_staged(a.rows, a.d)) {
       // One round of blocks: each SM's share of the rows is the same.

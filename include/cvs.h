@@ -235,6 +235,16 @@ cvs_status cvs_layer_norm_backward(const void* dy, int64_t dy_stride, const void
                                    void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Test hook for the failure path, as cvs_debug_stall_next_search: the next
+ * cvs_layer_norm or cvs_layer_norm_backward call with rows to work on, made on this
+ * host thread, copies none of them, and its waits give up after wait_cycles SM clocks
+ * (1000 .. 2^40). Calls whose kernel has no such wait (rows that are unaligned or wider
+ * than 1024; forward: fewer than 16384 rows) disarm it and return
+ * CVS_ERR_INVALID_ARGUMENT. The armed call's results are undefined.
+ */
+cvs_status cvs_debug_stall_next_norm(int64_t wait_cycles);
+
+/*
  * Copies half-precision rows of any alignment into rows that cvs_linear and
  * cvs_linear_backward accept: dst 16-byte aligned, dst_stride a multiple of 8 and
  * at least cols. Columns cols .. dst_stride-1 of dst may be written with zeros.

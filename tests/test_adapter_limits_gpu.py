@@ -21,6 +21,9 @@ def lib():
     lib = ctypes.CDLL(str(LIB))
     lib.cvs_last_error.restype = ctypes.c_char_p
     lib.cvs_layer_norm.argtypes = [vp, i32, i64, i32, i64, vp, vp, i32, f32, vp, i64, vp, vp, vp]
+    lib.cvs_layer_norm_backward.argtypes = [vp, i64, vp, i32, i64, i32, i64, vp, i32, vp, vp, vp, i64, vp, vp, vp, size, vp]
+    lib.cvs_debug_stall_next_norm.argtypes = [i64]
+    lib.cvs_poll_device_error.argtypes = [i32, ctypes.POINTER(ctypes.c_int)]
     lib.cvs_preference_loss.argtypes = [vp, i32, i64, vp, i32, i64, i64, i32, i32, vp, i64, i32, vp, vp, i64, i32, f32, f32,
                                         i32, vp, vp, vp, vp, i64, vp, size, vp]
     return lib
@@ -127,3 +130,47 @@ def test_preference_loss_of_two_widths_from_two_threads(lib):
         _, want, _ = oracle.preference(q, None, chosen, rejected, x, False, 1.0, 0.0, True)
         sizes = x.double().abs()[chosen][:, None] + x.double().abs()[rejected]
         oracle.close(margins, want, 150 * E * (sizes * q.double().abs()[:, None]).sum(2))
+
+
+# ---- waits that run out ------------------------------------------------------------------
+def norm_call(lib, x, y, dy=None, stats=None, ws=None):
+    rows, d = x.shape
+    s = torch.cuda.current_stream().cuda_stream
+    if dy is None:
+        mean, rstd = stats if stats else (None, None)
+        return lib.cvs_layer_norm(x.data_ptr(), 1, rows, d, d, None, None, 1, 1e-5, y.data_ptr(), d,
+                                  mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None, s)
+    return lib.cvs_layer_norm_backward(dy.data_ptr(), d, x.data_ptr(), 1, rows, d, d, None, 1, stats[0].data_ptr(),
+                                       stats[1].data_ptr(), y.data_ptr(), d, None, None, None, 0, s)
+
+
+def poll(lib):
+    code = ctypes.c_int(-1)
+    torch.cuda.synchronize()
+    return lib.cvs_poll_device_error(torch.cuda.current_device(), ctypes.byref(code)), code.value
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_a_layer_norm_wait_that_runs_out_is_reported(lib, backward):
+    """No row arrives, the waits end after 10^6 SM clocks: the device error word names the
+    site, and the next call is an ordinary one."""
+    x, dy = randn(16384, 768, dtype=torch.float16, seed=1), randn(16384, 768, dtype=torch.float16, seed=2)
+    y, stats = torch.empty_like(x), (torch.empty(16384, device="cuda"), torch.empty(16384, device="cuda"))
+    assert poll(lib) == (0, 0), "an earlier kernel left an error behind"
+    assert norm_call(lib, x, y, stats=stats) == 0 and poll(lib) == (0, 0)
+    args = (x, y, dy, stats) if backward else (x, y)
+    assert lib.cvs_debug_stall_next_norm(1_000_000) == 0
+    assert norm_call(lib, *args) == 0, lib.cvs_last_error()
+    assert poll(lib) == (5, 0x100 | (41 if backward else 42))
+    assert norm_call(lib, *args) == 0 and poll(lib) == (0, 0)
+    want_y, want_dx, *_ = oracle.layer_norm(x, None, None, 1e-5, dy)
+    oracle.close(y, want_dx if backward else want_y, 200 * E * (10 + want_y.abs()))
+
+
+def test_the_layer_norm_hook_refuses_kernels_without_a_ring(lib):
+    x = randn(100, 768, dtype=torch.float16, seed=1)
+    y = torch.empty_like(x)
+    assert lib.cvs_debug_stall_next_norm(1_000_000) == 0
+    assert norm_call(lib, x, y) == 1 and b"hook" in lib.cvs_last_error()
+    assert norm_call(lib, x, y) == 0 and poll(lib) == (0, 0)  # disarmed
+    assert lib.cvs_debug_stall_next_norm(10) == 1
