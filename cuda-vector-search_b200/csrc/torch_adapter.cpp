@@ -7,6 +7,7 @@
 
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -90,6 +91,14 @@ void check_capture(std::initializer_list<const Tensor*> inputs) {
                 "a parameter of a captured backward pass still belongs to an autograd graph made on another stream; "
                 "release that graph's outputs before the capture, or run it on the capture's stream");
   }
+}
+
+// The operators have no forward-mode derivative: an input's tangent would be lost.
+void check_tangents(std::initializer_list<const Tensor*> inputs, const char* what) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what,
+                ": forward-mode derivatives (torch.autograd.forward_ad) are not supported");
 }
 
 bool wants_grad(std::initializer_list<const Tensor*> inputs) {
@@ -196,6 +205,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   if (given(weight) && given(bias))
     TORCH_CHECK_TYPE(weight->scalar_type() == bias->scalar_type(), "layer_norm: weight and bias must have one dtype");
   const Tensor w = or_undefined(weight), b = or_undefined(bias);
+  check_tangents({&x, &w, &b}, "layer_norm");
   Tensor y;
   if (wants_grad({&x, &w, &b})) {
     check_capture({&x, &w, &b});
@@ -308,6 +318,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, int6
                       at::IntArrayRef(shape));
   }
   const Tensor b = or_undefined(bias), r = or_undefined(residual);
+  check_tangents({&x, &weight, &b, &r}, "linear");
   const Tensor r2 = r.defined() ? flat(r) : r;
   Tensor y;
   if (wants_grad({&x, &weight, &b, &r})) {
@@ -404,6 +415,7 @@ std::tuple<Tensor, Tensor> preference_loss(const Tensor& q, const OptTensor& ref
   TORCH_CHECK_VALUE(rejected.dim() == 2 && rejected.size(0) == q.size(0) && rejected.size(1) >= 1,
                     "preference_loss: rejected must be [b] or [b, r] with r >= 1");
   TORCH_CHECK_VALUE(smoothing >= 0 && smoothing <= 1, "preference_loss: label_smoothing must be in 0 .. 1");
+  check_tangents({&q}, "preference_loss");
   if (wants_grad({&q})) {
     check_capture({&q});
     const auto out = PreferenceFn::apply(q, ref.defined() ? OptTensor(ref) : OptTensor(), chosen, rejected, corpus, cosine,

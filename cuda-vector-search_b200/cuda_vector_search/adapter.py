@@ -5,8 +5,9 @@ fixed index, the operators it is made of, and its use in a search.
 trained with ``Index.preference_loss`` (queries, the rows users preferred, the rows they
 passed over) while the corpus stays as it is, and used with
 ``Index.search(queries, k, adapter=adapter)``. All operators run on this package's own
-kernels, on the current stream of their inputs' device; they are differentiable once,
-allocate through torch's caching allocator only, and can be captured into CUDA graphs.
+kernels, on the current stream of their inputs' device; they are differentiable once (in
+reverse mode: tangents of ``torch.autograd.forward_ad`` are refused), allocate through
+torch's caching allocator only, and can be captured into CUDA graphs.
 """
 
 from __future__ import annotations

@@ -255,8 +255,8 @@ class Index:
 
     # -- search -------------------------------------------------------------
     def _adapt(self, queries, adapter):
-        """The queries as ``adapter`` maps them (no gradients are kept)."""
-        q = self._query_tensor(queries)
+        """The queries as ``adapter`` maps them (no gradients and no tangents are kept)."""
+        q = torch.autograd.forward_ad.unpack_dual(self._query_tensor(queries)).primal
         with torch.no_grad(), torch.cuda.device(self.device):
             out = adapter(q if q.device == self.device else q.to(self.device, non_blocking=q.is_pinned()))
         return out

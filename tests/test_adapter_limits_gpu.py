@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import adapter_oracle as oracle
-from test_adapter_gpu import DTYPES, E, check_norm, cvs, ids, randn  # noqa: F401  (cvs: the fixture)
+from test_adapter_gpu import DTYPES, E, check_norm, cvs, ids, make_index, randn  # noqa: F401  (cvs: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -174,3 +174,26 @@ def test_the_layer_norm_hook_refuses_kernels_without_a_ring(lib):
     assert norm_call(lib, x, y) == 1 and b"hook" in lib.cvs_last_error()
     assert norm_call(lib, x, y) == 0 and poll(lib) == (0, 0)  # disarmed
     assert lib.cvs_debug_stall_next_norm(10) == 1
+
+
+# ---- forward derivatives ------------------------------------------------------------
+def test_forward_derivatives_are_refused(cvs):
+    """A tangent would be lost: every differentiable input that carries one is refused."""
+    import torch.autograd.forward_ad as fw
+
+    x, w, b = randn(9, 64, dtype=torch.float16, seed=1), randn(64, 64, dtype=torch.float16, seed=2), randn(64, dtype=torch.float16, seed=3)
+    index = make_index(cvs, 100, 64, "ip")
+    c, rej = ids(100, 9, seed=4), ids(100, 9, seed=5)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: cvs.layer_norm(dual(x)), lambda: cvs.layer_norm(x, dual(b)), lambda: cvs.layer_norm(x, b, dual(b)),
+                     lambda: cvs.linear(dual(x), w), lambda: cvs.linear(x, dual(w)), lambda: cvs.linear(x, w, dual(b)),
+                     lambda: cvs.linear(x, w, residual=dual(x)), lambda: index.preference_loss(dual(x), c, rej),
+                     lambda: cvs.layer_norm(dual(x).requires_grad_())):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        index.preference_loss(x, c, rej, reference=dual(x))  # a constant by definition
+        a = cvs.Adapter(64, device="cuda")
+        v, i = index.search(dual(x), 3, adapter=a)  # a search has no derivative
+    v2, i2 = index.search(x, 3, adapter=a)
+    assert torch.equal(v, v2) and torch.equal(i, i2)
