@@ -31,7 +31,8 @@
 // are too few queries to fill the GPU with one warp each; the shares are added
 // through shared memory in a fixed order. Ids below zero mark absent rows (a query
 // without a chosen row, a shorter list of rejected ones): their pairs give margin
-// zero and do not count. An id that is not a row of the corpus reads nothing and
+// zero and do not count, and no value that lies there (in a padded query, in a chosen row
+// whose rejected rows are all absent) reaches a result, NaN and infinity included. An id that is not a row of the corpus reads nothing and
 // makes its pair's margin NaN, and so the loss.
 #include "cvs_device.cuh"
 #include "cvs_elem.cuh"
@@ -209,6 +210,7 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
   // [warps][2 stages][rows] row buffers, then (several warps a query) the gradient's shares [warps][d_pad].
   extern __shared__ __align__(128) uint8_t rows_s[];
   __shared__ float2 totals[kPrefWarps];
+  __shared__ int present[kPrefWarps];  // whether the warp's share of the query has a pair
   __shared__ __align__(8) uint64_t bars[kPrefWarps][2];
   __shared__ int abort_s;
   const int lane = threadIdx.x & 31;
@@ -251,6 +253,7 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
     }
     Raw8<__half> xc[CPL];
     float slopes = 0.f;  // sum of the slopes
+    bool any = false;    // this warp has a pair
     if (live) {
       if (q + step < a.b) {
         prefetch_row(a.q, a.q_dtype, (q + step) * a.q_stride, a.d, lane);
@@ -303,6 +306,7 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
       for (int k = 0; k < mine; ++k) {
         const bool gone = gone_c || stream.gone();
         const bool row = row_c && stream.there();
+        any |= !gone;
         float m = gone ? 0.f : __int_as_float(0x7fffffff);
         if (row && !gone) {
           Pair x[CPL][4];
@@ -354,7 +358,7 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
       }
     }
     if (a.grad == nullptr) continue;
-    if (live) {
+    if (any) {  // else zeros
 #pragma unroll
       for (int j = 0; j < CPL; ++j) {
 #pragma unroll
@@ -362,6 +366,7 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
       }
     }
     if (wpq > 1) {
+      if (lane == 0) present[warp] = any;
       if (live && share != 0) {
         float4* out = reinterpret_cast<float4*>(shares + static_cast<size_t>(warp) * a.d_pad);
 #pragma unroll
@@ -381,6 +386,7 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
       __syncthreads();
       if (live && share == 0) {
         for (int w = 1; w < wpq; ++w) {
+          any |= present[warp + w] != 0;
           const float4* in = reinterpret_cast<const float4*>(shares + static_cast<size_t>(warp + w) * a.d_pad);
 #pragma unroll
           for (int j = 0; j < CPL; ++j) {
@@ -398,7 +404,7 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
       __syncthreads();  // the shares are read before the next round writes them
     }
     if (!live || share != 0) continue;
-    if (a.cosine) {
+    if (a.cosine && any) {
       Pair u[CPL][4];
       load_pairs<CPL>(a.q, a.q_dtype, q * a.q_stride, a.d, a.q_vec, lane, u);
       Pair dot = both(0.f);

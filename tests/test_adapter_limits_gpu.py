@@ -197,3 +197,38 @@ def test_forward_derivatives_are_refused(cvs):
         v, i = index.search(dual(x), 3, adapter=a)  # a search has no derivative
     v2, i2 = index.search(x, 3, adapter=a)
     assert torch.equal(v, v2) and torch.equal(i, i2)
+
+
+# ---- values at absent rows -------------------------------------------------------------
+@pytest.mark.parametrize("metric", ["cosine", "ip"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("b,r", [(6, 1), (6, 9), (3000, 2)])
+def test_preference_absent_pairs_ignore_what_lies_there(cvs, metric, bad, b, r):
+    """Padding holds anything: a query without a pair, a chosen row whose rejected rows are
+    all absent. Its gradient is zero and nothing else changes."""
+    x = randn(300, 96, dtype=torch.float16, seed=1, scale=0.3)
+    x[299] = bad
+    index = cvs.Index(torch.nn.functional.pad(x, (0, 32)), metric=metric, copy=False)  # as it is: not normalised again
+    q, ref = randn(b, 96, dtype=torch.float32, seed=2), randn(b, 96, dtype=torch.float32, seed=3)
+    q, ref = torch.nn.functional.pad(q, (0, 32)), torch.nn.functional.pad(ref, (0, 32))
+    c, rej = ids(299, b, seed=4), ids(299, b, r, seed=5)
+    q[1], ref[1], c[1] = bad, bad, -1           # a padded query
+    q[2], rej[2] = bad, -1                      # a query whose rejected rows are all absent
+    c[4], rej[4] = 299, -1                      # a bad chosen row in front of absent ones
+    c[5], rej[5] = -1, 299                      # bad rejected rows behind an absent one
+    want_q = q.clone()
+    want_q[[1, 2]] = 0.5
+
+    def run(q, ref, c, rej):
+        q = q.detach().requires_grad_()
+        loss, m = index.preference_loss(q, c, rej, reference=ref, scale=3.0, return_margins=True)
+        return (loss.detach(), m, *torch.autograd.grad(loss, q))
+
+    got = run(q, ref, c, rej)
+    ref2, c2, rej2 = ref.clone(), c.clone(), rej.clone()
+    ref2[1], c2[4], rej2[5] = 0.5, 0, 0
+    want = run(want_q, ref2, c2, rej2)
+    assert all(torch.isfinite(t).all() for t in got)
+    assert (got[2][[1, 2, 4, 5]] == 0).all()
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
