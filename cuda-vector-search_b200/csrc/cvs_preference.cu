@@ -49,6 +49,7 @@ constexpr int kPrefThreads = 256;
 constexpr int kPrefWarps = kPrefThreads / 32;
 constexpr int kPrefStageRows = 8;  // most row buffers of a warp's stage
 constexpr int kAbsent = -1, kOutside = -2;  // what a position may hold instead of a row
+constexpr float kLog2E = 1.44269504088896341f, kLog2ELow = 1.92596299e-08f, kLn2 = 0.69314718056f;  // log2(e) = kLog2E + kLog2ELow
 
 // This lane's columns of a query row as pairs of fp32 (zeros outside).
 template <class T, int CPL>
@@ -324,8 +325,13 @@ __global__ void __launch_bounds__(kPrefThreads, CPL <= 4 ? 2 : 1) preference_ker
           }
           m = a.scale * (dot_c - warp_sum(pair_total(pair_add(dot, dot2))));
           if (a.grad != nullptr) {
-            // sigmoid(-m) from e^-|m| (2 ulp each: exponential, reciprocal).
-            const float e = exp2_approx(-1.4426950408889634f * fabsf(m));
+            // sigmoid(-m) from e^-|m| (exponential 2 ulp, reciprocal 1). The exponent is |m| / ln 2
+            // to more than fp32's digits: p, and what p misses as a factor 1 + rest ln 2 -- the
+            // rounding of p alone would cost a confident pair's slope |m| / 2 ulp.
+            const float p = -kLog2E * fabsf(m);
+            const float rest = fmaf(-kLog2E, fabsf(m), -p) - kLog2ELow * fabsf(m);
+            const float e0 = exp2_approx(p);
+            const float e = e0 == 0.f ? 0.f : fmaf(e0, rest * kLn2, e0);  // (an infinite margin: rest is NaN)
             const float below = (m > 0.f ? e : 1.f) * rcp_approx(1.f + e);
             const float slope = (a.smoothing - below) * a.scale;
             slopes += slope;

@@ -232,3 +232,35 @@ def test_preference_absent_pairs_ignore_what_lies_there(cvs, metric, bad, b, r):
     assert (got[2][[1, 2, 4, 5]] == 0).all()
     for g, w in zip(got, want):
         assert torch.equal(g, w)
+
+
+def test_preference_slopes_of_confident_pairs(cvs):
+    """Margins that are exact (one column, one product): an fp32 gradient is then off by the
+    slope's own roundings alone: exponential 4 e (2 ulp) and its argument's rest e, the sum
+    1 + e^-|m| e, reciprocal 2 e (1 ulp), their product e; the other factors are one."""
+    n = 80
+    x = torch.zeros(2, 64, dtype=torch.float16, device="cuda")
+    x[0, 0] = 1.0
+    index = cvs.Index(x, metric="ip", copy=False)
+    q = torch.zeros(n, 64, device="cuda")
+    q[:, 0] = torch.linspace(-80.0, 80.0, n, device="cuda") + randn(n, dtype=torch.float32, seed=1)
+    q.requires_grad_()
+    loss = index.preference_loss(q, torch.zeros(n, dtype=torch.int64, device="cuda"), torch.ones(n, dtype=torch.int64, device="cuda"),
+                                 reduction="sum")
+    (dq,) = torch.autograd.grad(loss, q)
+    oracle.close(dq[:, 0], -torch.sigmoid(-q.detach().double()[:, 0]), 9 * E * torch.sigmoid(-q.detach().double()[:, 0]))
+
+
+def test_preference_infinite_margins(cvs):
+    """A margin past fp32: the pair's slope is 0 or -scale, not NaN."""
+    x = torch.zeros(2, 64, dtype=torch.float16, device="cuda")
+    x[0, 0] = 60000.0
+    index = cvs.Index(x, metric="ip", copy=False)
+    q = torch.zeros(2, 64, device="cuda")
+    q[0, 0], q[1, 0] = 1e38, -1e38
+    q.requires_grad_()
+    c, rej = torch.zeros(2, dtype=torch.int64, device="cuda"), torch.ones(2, dtype=torch.int64, device="cuda")
+    loss, m = index.preference_loss(q, c, rej, reduction="sum", label_smoothing=0.25, return_margins=True)
+    (dq,) = torch.autograd.grad(loss, q)
+    assert m[0, 0] == float("inf") and m[1, 0] == float("-inf") and torch.isinf(loss)
+    assert dq[0, 0] == 0.25 * 60000.0 and dq[1, 0] == -0.75 * 60000.0
