@@ -264,3 +264,28 @@ def test_preference_infinite_margins(cvs):
     (dq,) = torch.autograd.grad(loss, q)
     assert m[0, 0] == float("inf") and m[1, 0] == float("-inf") and torch.isinf(loss)
     assert dq[0, 0] == 0.25 * 60000.0 and dq[1, 0] == -0.75 * 60000.0
+
+
+# ---- activations' tails ---------------------------------------------------------------
+@pytest.mark.parametrize("m", [1, 2, 300])
+def test_gelu_goes_to_zero(cvs, m):
+    """Far below zero a bf16 GELU and its slope follow z Phi(z) down to fp32's smallest
+    numbers instead of stopping at their value at -6: to 1e-3 above -9, 1e-2 above -11, and
+    zero (or below 1e-27, where fp32 ends) beyond."""
+    t = torch.bfloat16
+    zs = torch.tensor([-5.0, -5.9375, -6.0, -6.0625, -6.5, -7.0, -8.0, -9.0, -10.0, -11.0, -12.0, -13.0, -14.0, -20.0, -50.0, -1e4])
+    w = torch.zeros(16, 8, dtype=t, device="cuda")
+    w[:, 0] = zs.to(t).cuda()
+    x = torch.zeros(m, 8, dtype=t, device="cuda")
+    x[:, 0] = 1.0
+    y = cvs.linear(x, w, activation="gelu")
+    z = w.double()[:, 0].expand(m, 16)
+    want, slope = oracle.act(z, "gelu")
+    rel = torch.where(z >= -9, 1e-3, torch.where(z >= -11, 1e-2, 1.0))
+    oracle.close(y, want, rel * want.abs() + 1e-37)
+    assert (y[:, z[0] <= -14] == 0).all()
+    one = torch.zeros(1, 8, dtype=t, device="cuda")
+    one[0, 0] = 1.0
+    x = w.detach().clone().requires_grad_()  # rows with z in the first column: one output, its slope in dx's first column
+    (dx,) = torch.autograd.grad(cvs.linear(x, one, activation="gelu"), x, torch.ones(16, 1, dtype=t, device="cuda"))
+    oracle.close(dx[:, 0], slope[0], (rel[0] + 2.0**-8) * slope[0].abs() + 1e-37)
