@@ -56,7 +56,7 @@ cvs_status check_norm(int dtype, int64_t rows, int d, int64_t x_stride, int weig
 // ---- linear ---------------------------------------------------------------------
 cvs_status check_linear(int activation, int dtype, int64_t m, int n, int k) {
   if (m < 0 || m >= INT_MAX) return fail(CVS_ERR_INVALID_ARGUMENT, "row count %lld out of range", (long long)m);
-  if (n < 1 || k < 1 || n > (1 << 24) || k > (1 << 24))
+  if (n < 1 || k < 1 || n > CVS_MAX_LAYER_WIDTH || k > CVS_MAX_LAYER_WIDTH)
     return fail(CVS_ERR_INVALID_ARGUMENT, "layer widths must be in 1 .. 2^24 (got %d x %d)", n, k);
   if (activation < CVS_ACT_NONE || activation > CVS_ACT_SILU)
     return fail(CVS_ERR_INVALID_ARGUMENT, "unknown activation %d", activation);
@@ -556,7 +556,8 @@ cvs_status cvs_preference_loss_workspace_size(int64_t b, int r, size_t* bytes) {
   if (!bytes) return fail(CVS_ERR_INVALID_ARGUMENT, "bytes must not be null");
   *bytes = 0;
   if (b < 0 || b >= INT_MAX) return fail(CVS_ERR_INVALID_ARGUMENT, "query count out of range");
-  if (r < 1) return fail(CVS_ERR_INVALID_ARGUMENT, "at least one rejected row per query");
+  if (r < 1 || r > CVS_MAX_REJECTED)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "rejected rows per query must be in 1 .. %d (got %d)", CVS_MAX_REJECTED, r);
   if (b == 0) return CVS_OK;
   DeviceInfo dev;
   const cvs_status st = device_info(&dev);
@@ -572,7 +573,8 @@ cvs_status cvs_preference_loss(const void* q, int q_dtype, int64_t q_stride, con
                                float* margins, float* grad, int64_t grad_stride, void* workspace,
                                size_t workspace_bytes, void* stream) {
   if (b < 0 || b >= INT_MAX) return fail(CVS_ERR_INVALID_ARGUMENT, "query count %lld out of range", (long long)b);
-  if (r < 1) return fail(CVS_ERR_INVALID_ARGUMENT, "at least one rejected row per query");
+  if (r < 1 || r > CVS_MAX_REJECTED)
+    return fail(CVS_ERR_INVALID_ARGUMENT, "rejected rows per query must be in 1 .. %d (got %d)", CVS_MAX_REJECTED, r);
   if (n < 1 || n >= INT_MAX)
     return fail(CVS_ERR_INVALID_ARGUMENT, "corpus must have 1 .. 2^31-1 rows (got %lld)", (long long)n);
   if (d_pad < CVS_PAD || d_pad % CVS_PAD != 0 || d_pad > 2048)

@@ -300,7 +300,9 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, int6
                    "linear: x must be float16 or bfloat16, not ", x.scalar_type());
   check_device(weight, "linear: weight", x);
   TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type(), "linear: weight must have x's dtype");
-  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(1) >= 1, "linear: weight must be [n, k]");
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(1) >= 1 &&
+                        weight.size(0) <= CVS_MAX_LAYER_WIDTH && weight.size(1) <= CVS_MAX_LAYER_WIDTH,
+                    "linear: weight must be [n, k], both at most ", CVS_MAX_LAYER_WIDTH);
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == weight.size(1), "linear: x must be [..., ", weight.size(1), "]");
   TORCH_CHECK_VALUE(activation >= CVS_ACT_NONE && activation <= CVS_ACT_SILU, "linear: unknown activation");
   const int64_t n = weight.size(0);
@@ -412,8 +414,9 @@ std::tuple<Tensor, Tensor> preference_loss(const Tensor& q, const OptTensor& ref
   TORCH_CHECK_TYPE(chosen.scalar_type() == torch::kLong && rejected.scalar_type() == torch::kLong,
                    "preference_loss: chosen and rejected must be int64 row ids");
   TORCH_CHECK_VALUE(chosen.dim() == 1 && chosen.size(0) == q.size(0), "preference_loss: chosen must be [b]");
-  TORCH_CHECK_VALUE(rejected.dim() == 2 && rejected.size(0) == q.size(0) && rejected.size(1) >= 1,
-                    "preference_loss: rejected must be [b] or [b, r] with r >= 1");
+  TORCH_CHECK_VALUE(rejected.dim() == 2 && rejected.size(0) == q.size(0) && rejected.size(1) >= 1 &&
+                        rejected.size(1) <= CVS_MAX_REJECTED,
+                    "preference_loss: rejected must be [b] or [b, r] with r in 1 .. ", CVS_MAX_REJECTED);
   TORCH_CHECK_VALUE(smoothing >= 0 && smoothing <= 1, "preference_loss: label_smoothing must be in 0 .. 1");
   check_tangents({&q}, "preference_loss");
   if (wants_grad({&q})) {

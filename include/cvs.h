@@ -203,6 +203,8 @@ cvs_status cvs_set_profile_events(void* start_event, void* stop_event);
  * ------------------------------------------------------------------------- */
 
 #define CVS_MAX_NORM_WIDTH 8192  /* columns of a layer norm */
+#define CVS_MAX_LAYER_WIDTH (1 << 24)  /* n and k of a linear layer */
+#define CVS_MAX_REJECTED (1 << 30)     /* rejected rows per query of a preference loss */
 #define CVS_LINEAR_SMALL_ROWS 8  /* rows up to which cvs_linear takes operands of any alignment */
 
 typedef enum cvs_activation {

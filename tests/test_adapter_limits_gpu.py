@@ -289,3 +289,17 @@ def test_gelu_goes_to_zero(cvs, m):
     x = w.detach().clone().requires_grad_()  # rows with z in the first column: one output, its slope in dx's first column
     (dx,) = torch.autograd.grad(cvs.linear(x, one, activation="gelu"), x, torch.ones(16, 1, dtype=t, device="cuda"))
     oracle.close(dx[:, 0], slope[0], (rel[0] + 2.0**-8) * slope[0].abs() + 1e-37)
+
+
+# ---- counts past 32 bits ---------------------------------------------------------------
+def test_counts_past_32_bits_are_refused(cvs):
+    """A count of columns or rows is never cut to its low 32 bits."""
+    x = randn(4, 1, dtype=torch.float16, seed=1)
+    with pytest.raises(ValueError, match="at most"):
+        cvs.linear(x, x[:1].expand((1 << 32) + 5, 1))
+    with pytest.raises(ValueError, match="at most"):
+        cvs.linear(x[:1].expand(4, (1 << 32) + 5), x[:1].expand(3, (1 << 32) + 5))
+    index = make_index(cvs, 100, 64, "ip")
+    with pytest.raises(ValueError, match="rejected"):
+        index.preference_loss(randn(4, 64, dtype=torch.float32, seed=1), ids(100, 4, seed=2),
+                              ids(100, 4, 1, seed=3).expand(4, (1 << 32) + 1))
