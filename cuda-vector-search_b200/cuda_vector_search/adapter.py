@@ -51,7 +51,9 @@ class Adapter(torch.nn.Module):
         dim: embedding width.
         hidden: width of the hidden layer (default: twice the embedding's).
         activation: "gelu", "relu", "silu" or "none".
-        dtype: float16 or bfloat16, of the parameters and of the computation.
+        dtype: float16 or bfloat16, of the parameters and of the computation. An
+            optimizer's small steps are lost in either: let it work on float32 copies of
+            the parameters and copy them back after each step.
     """
 
     def __init__(self, dim: int, hidden: int | None = None, activation: str = "gelu", eps: float = 1e-5,

@@ -303,3 +303,30 @@ def test_counts_past_32_bits_are_refused(cvs):
     with pytest.raises(ValueError, match="rejected"):
         index.preference_loss(randn(4, 64, dtype=torch.float32, seed=1), ids(100, 4, seed=2),
                               ids(100, 4, 1, seed=3).expand(4, (1 << 32) + 1))
+
+
+# ---- training as documented ------------------------------------------------------------
+def test_the_documented_training_loop(cvs):
+    """README's loop as it stands: the fp32 copies take every step, the parameters are their
+    rounded values, and the gradient the loop ends on is the adapter's own."""
+    text = (LIB.parent.parent.parent / "README.md").read_text()
+    code = text[text.index("from cuda_vector_search import Adapter, Index") :]
+    code = code[: code.index("```")]
+    index = make_index(cvs, 2000, 768, "cosine")
+    q = randn(100, 768, dtype=torch.bfloat16, seed=2)
+    batch = (q, ids(2000, 100, seed=3), ids(2000, 100, 4, seed=4, gone=0.2))
+    torch.manual_seed(0)
+    names = {"torch": torch, "index": index, "batches": [batch] * 20, "q": q}
+    exec(code, names)
+    adapter, master, params = names["adapter"], names["master"], names["params"]
+    torch.manual_seed(0)
+    start = cvs.Adapter(768, dtype=torch.bfloat16, device="cuda")
+    for m, p, p0 in zip(master, params, start.parameters()):
+        assert m.dtype == torch.float32 and torch.isfinite(m).all() and torch.equal(p.detach(), m.to(p.dtype))
+        # 20 AdamW steps move a value by at most 20 lr (1 + its decay) or so, and move it at all.
+        moved = (m - p0.detach().float()).abs()
+        assert (moved > 0).all() and moved.max() < 20 * 1e-4 * 2
+    loss = index.preference_loss(adapter(q), *batch[1:], reference=q, scale=10.0)
+    for g, p in zip(torch.autograd.grad(loss, params), params):
+        assert torch.isfinite(g).all() and (g != 0).any() and g.shape == p.shape
+    assert names["ids"].shape == (100, 10)
