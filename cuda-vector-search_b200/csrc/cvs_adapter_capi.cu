@@ -72,24 +72,6 @@ cvs_status check_operand(const void* p, int64_t stride, int64_t width, const cha
   return CVS_OK;
 }
 
-// Tensor map of a half-precision matrix [rows][cols], rows `stride` elements apart,
-// in boxes of 64 columns (one 128-byte swizzled row) x box_rows rows.
-cvs_status make_half_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int64_t cols, int64_t stride,
-                         int box_rows) {
-  auto fn = encode_fn();
-  if (!fn) return fail(CVS_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
-  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
-  cuuint32_t estr[2] = {1, 1};
-  const CUresult r =
-      fn(map, dtype == CVS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(CVS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
-  return CVS_OK;
-}
-
 // A product's operand: stored [mn][k] (K-major) or [k][mn] (MN-major).
 struct Operand {
   const void* p;

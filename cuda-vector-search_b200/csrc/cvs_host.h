@@ -1,5 +1,5 @@
 // Host helpers of the C ABI's translation units: status and message of a failed
-// call, the current device, the driver's tensor-map encoder.
+// call, the current device, tensor maps.
 #pragma once
 
 #include <cudaTypedefs.h>
@@ -23,7 +23,9 @@ cvs_status cuda_fail(cudaError_t e, const char* what);
 // The current device; CVS_ERR_UNSUPPORTED unless it is an sm_100 GPU.
 cvs_status device_info(DeviceInfo* out, int* dev_out = nullptr);
 
-// cuTensorMapEncodeTiled, or null when the driver does not have it.
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
+// Tensor map of a half-precision matrix [rows][cols], rows `stride` elements apart, in
+// boxes of 64 columns (one 128-byte swizzled row) x box_rows rows. Works in any host thread.
+cvs_status make_half_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int64_t cols, int64_t stride,
+                         int box_rows);
 
 }  // namespace cvs

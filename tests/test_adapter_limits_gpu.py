@@ -1,6 +1,8 @@
 """The adapter's operators where a first set of sizes did not look."""
 
 import ctypes
+import subprocess
+import sys
 import threading
 from pathlib import Path
 
@@ -22,11 +24,19 @@ def lib():
     lib.cvs_last_error.restype = ctypes.c_char_p
     lib.cvs_layer_norm.argtypes = [vp, i32, i64, i32, i64, vp, vp, i32, f32, vp, i64, vp, vp, vp]
     lib.cvs_layer_norm_backward.argtypes = [vp, i64, vp, i32, i64, i32, i64, vp, i32, vp, vp, vp, i64, vp, vp, vp, size, vp]
+    lib.cvs_linear.argtypes = [vp, i64, vp, i64, vp, vp, i64, i32, i32, i64, i32, i32, vp, i64, vp, i64, vp]
+    lib.cvs_linear_backward_workspace_size.argtypes = [i32, i64, i32, i32, ctypes.POINTER(size)]
+    lib.cvs_linear_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i64, i32, i32, vp, i64, vp, i64, vp, vp,
+                                        size, vp]
     lib.cvs_debug_stall_next_norm.argtypes = [i64]
     lib.cvs_poll_device_error.argtypes = [i32, ctypes.POINTER(ctypes.c_int)]
     lib.cvs_preference_loss.argtypes = [vp, i32, i64, vp, i32, i64, i64, i32, i32, vp, i64, i32, vp, vp, i64, i32, f32, f32,
                                         i32, vp, vp, vp, vp, i64, vp, size, vp]
     return lib
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
 
 
 # ---- layer norm -------------------------------------------------------------------
@@ -71,7 +81,10 @@ def in_threads(*calls, repeats=4000):
     def work(j):
         start.wait()
         for _ in range(repeats):
-            why = calls[j]()
+            try:
+                why = calls[j]()
+            except RuntimeError as e:
+                why = str(e)
             if why:
                 errors[j] = why
                 return
@@ -135,7 +148,7 @@ def test_preference_loss_of_two_widths_from_two_threads(lib):
 # ---- waits that run out ------------------------------------------------------------------
 def norm_call(lib, x, y, dy=None, stats=None, ws=None):
     rows, d = x.shape
-    s = torch.cuda.current_stream().cuda_stream
+    s = stream()
     if dy is None:
         mean, rstd = stats if stats else (None, None)
         return lib.cvs_layer_norm(x.data_ptr(), 1, rows, d, d, None, None, 1, 1e-5, y.data_ptr(), d,
@@ -330,3 +343,33 @@ def test_the_documented_training_loop(cvs):
     for g, p in zip(torch.autograd.grad(loss, params), params):
         assert torch.isfinite(g).all() and (g != 0).any() and g.shape == p.shape
     assert names["ids"].shape == (100, 10)
+
+
+# ---- host threads that have made no CUDA call yet ----------------------------------------
+def test_linear_from_a_new_thread(cvs):
+    """Nothing has bound the device to the thread before its first call."""
+    x, w = randn(700, 64, dtype=torch.float16, seed=1), randn(64, 64, dtype=torch.float16, seed=2)
+    spare = cvs.linear(x, w)
+    want = spare.clone()
+    del spare  # the thread's result takes this block: no allocation binds the device either
+    torch.cuda.synchronize()
+    assert in_threads(lambda: None if torch.equal(cvs.linear(x, w), want) else "differs", repeats=1) == [None]
+
+
+def test_backward_as_the_first_call_of_the_autograd_thread():
+    """In a fresh process: a backward pass without activation starts with its product."""
+    code = """
+import torch, cuda_vector_search as cvs
+x = torch.ones(700, 64, dtype=torch.float16, device="cuda", requires_grad=True)
+w = torch.ones(64, 64, dtype=torch.float16, device="cuda")
+y = cvs.linear(x, w)
+dy = torch.ones_like(y)
+spare = [torch.empty_like(y) for _ in range(4)]  # blocks for the backward pass to reuse
+del spare
+torch.cuda.synchronize()
+(dx,) = torch.autograd.grad(y, x, dy)
+assert (dx == 64).all()
+"""
+    root = LIB.parent.parent
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=200)
+    assert run.returncode == 0, run.stderr[-2000:]
