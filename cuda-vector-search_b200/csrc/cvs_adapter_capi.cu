@@ -84,10 +84,13 @@ cvs_status operand_map(CUtensorMap* map, const Operand& o, int dtype, int64_t mn
                     : make_half_map(map, o.p, dtype, mn, k, o.stride, box_mn);
 }
 
-// Rows a tensor map can describe, and the map of what the epilogue moves.
+// Rows a tensor map can describe, and the map of what the epilogue moves. A store writes
+// whole 16-byte units (zeros behind the width), so only whole rows of them are stored
+// through a map; loads read zeros behind the width.
 bool mappable(const void* p, int64_t stride, int64_t width) {
   return p && aligned16(p) && stride % 8 == 0 && stride >= width;
 }
+bool storable(const void* p, int64_t stride, int64_t width) { return mappable(p, stride, width) && width % 8 == 0; }
 cvs_status block_map(CUtensorMap* map, const void* p, int dtype, int64_t rows, int64_t cols, int64_t stride) {
   return make_half_map(map, p, dtype, rows, cols, stride, 32);
 }
@@ -397,7 +400,7 @@ cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_
   a.act = activation;
   p.out = y;
   p.ld_out = y_stride;
-  p.vec_out = mappable(y, y_stride, n);
+  p.vec_out = storable(y, y_stride, n);
   p.bias = bias;
   p.residual = residual;
   p.ld_res = residual_stride;
@@ -488,7 +491,7 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
       p.a_mn = p.b_mn = 1;
       p.out = dw;
       p.ld_out = dw_stride;
-      p.vec_out = mappable(dw, dw_stride, k);
+      p.vec_out = storable(dw, dw_stride, k);
       p.partial = p.splits > 1 ? reinterpret_cast<float*>(base + plan.dw_offset) : nullptr;
       if ((st = operand_map(&maps.a[i], {dz.p, dz.stride, true}, dtype, n, m, 64)) != CVS_OK) return st;
       if ((st = operand_map(&maps.b[i], {x, x_stride, true}, dtype, k, m, 64)) != CVS_OK) return st;
@@ -501,7 +504,7 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
       p.b_mn = 1;
       p.out = dx;
       p.ld_out = dx_stride;
-      p.vec_out = mappable(dx, dx_stride, k);
+      p.vec_out = storable(dx, dx_stride, k);
       if ((st = operand_map(&maps.a[i], dz, dtype, m, n, 128)) != CVS_OK) return st;
       if ((st = operand_map(&maps.b[i], {w, w_stride, true}, dtype, k, n, 64)) != CVS_OK) return st;
       if (p.vec_out && (st = block_map(&maps.out[i], dx, dtype, m, k, dx_stride)) != CVS_OK) return st;

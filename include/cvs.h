@@ -258,7 +258,8 @@ cvs_status cvs_align_rows(const void* src, int64_t src_stride, int dtype, int64_
  * y[m][n] = act(x[m][k] . w[n][k]^T + bias) + residual, dtype CVS_F16 or CVS_BF16
  * for every operand. bias [n] and residual [m][n] may be NULL. z, unless NULL
  * (and unless there is no activation), receives x . w^T + bias as fp16 (also for
- * CVS_BF16) for cvs_linear_backward: 16-byte aligned, z_stride a multiple of 8.
+ * CVS_BF16) for cvs_linear_backward: 16-byte aligned, z_stride a multiple of 8; its
+ * columns from n up to the next multiple of 8 may be written.
  * x and w: 16-byte aligned with strides a multiple of 8 unless m is at most
  * CVS_LINEAR_SMALL_ROWS; y, bias and residual may have any alignment.
  */

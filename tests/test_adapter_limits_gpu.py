@@ -373,3 +373,102 @@ assert (dx == 64).all()
     root = LIB.parent.parent
     run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=200)
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+# ---- the C ABI's own strides ----------------------------------------------------------
+FILL = 77.0
+
+
+def padded(rows, cols, stride, dtype, offset=0, values=None):
+    """(buffer, view): rows `stride` apart in a buffer of FILL that goes on behind the last row."""
+    buf = torch.full((offset + (rows + 2) * stride,), FILL, dtype=dtype, device="cuda")
+    view = buf[offset : offset + rows * stride].view(rows, stride)[:, :cols]
+    if values is not None:
+        view.copy_(values)
+    return buf, view
+
+
+def untouched(buf, view, also=0):
+    """Everything outside the view (and `also` columns behind it) is as it was."""
+    kept = torch.ones_like(buf, dtype=torch.bool)
+    rows, cols = view.shape
+    kept.as_strided((rows, cols + also), (view.stride(0), 1), view.storage_offset()).fill_(False)
+    return bool((buf[kept] == FILL).all())
+
+
+@pytest.mark.parametrize("activation", ["none", "relu", "gelu"])
+@pytest.mark.parametrize("more,offset", [(8, 0), (16, 8), (5, 1)])  # aligned and other strides, past the width
+@pytest.mark.parametrize("m,k,n", [(1, 64, 72), (2, 72, 65), (40, 256, 72), (40, 256, 65), (700, 64, 72), (700, 64, 65), (700, 65, 200),
+                                   (300, 391, 130)])
+def test_c_abi_linear_strides(lib, m, k, n, more, offset, activation):
+    t, act = torch.float16, ("none", "relu", "gelu").index(activation)
+    up8 = lambda v: (v + 7) // 8 * 8  # noqa: E731
+    _, x = padded(m, k, up8(k) + 8, t, 0, randn(m, k, dtype=t, seed=1))
+    _, w = padded(n, k, up8(k) + 16, t, 0, randn(n, k, dtype=t, seed=2, scale=k**-0.5))
+    b = randn(n, dtype=t, seed=3)
+    aligned = more % 8 == 0
+    s_out = (up8(n) if aligned else n) + more
+    _, res = padded(m, n, s_out, t, offset, randn(m, n, dtype=t, seed=4))
+    ybuf, y = padded(m, n, s_out, t, offset)
+    zbuf, z = padded(m, n, up8(n) + 8, t)
+    keep = activation != "none"
+    st = lib.cvs_linear(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), b.data_ptr(), res.data_ptr(), s_out, act, 1, m, n, k,
+                        y.data_ptr(), s_out, z.data_ptr() if keep else None, z.stride(0) if keep else 0, stream())
+    assert st == 0, lib.cvs_last_error()
+    want, zd, slope, scale = oracle.linear(x, w, b, activation, res)
+    dz_z = (k / 8 + 16) * E * scale
+    oracle.close(y, want, 1.13 * dz_z + 16 * E * zd.abs() + 2 * E * want.abs())
+    assert untouched(ybuf, y)
+    if keep:
+        oracle.close(z, zd, dz_z)
+        assert untouched(zbuf, z, up8(n) - n)
+    # Backward: all gradients, and each product alone.
+    _, dy = padded(m, n, s_out, t, offset, randn(m, n, dtype=t, seed=5))
+    nbytes = size()
+    assert lib.cvs_linear_backward_workspace_size(act, m, n, k, ctypes.byref(nbytes)) == 0
+    ws = torch.empty(max(nbytes.value, 256), dtype=torch.uint8, device="cuda")
+    s_dx = k + more
+    if keep:
+        s_err = (zd.abs() <= dz_z).double() if activation == "relu" else 0.8 * (2.0**-11 * zd.abs() + 2.0**-25 + dz_z) + 16 * E
+    else:
+        s_err = torch.zeros_like(zd)
+    dyd, wd, xd = dy.double(), w.double(), x.double()
+    dz = dyd * slope
+    dz_err = dyd.abs() * s_err + (2.0**-11 * dz.abs() + 2.0**-25 if keep else 0)
+    for wanted in ("xwb", "x", "w", "b"):
+        dxb, dx = padded(m, k, s_dx, t, offset)
+        dwb, dw = padded(n, k, s_dx, t, offset)
+        db = torch.full((n + 8,), FILL, dtype=t, device="cuda")
+        p = lambda c, v: v.data_ptr() if c in wanted else None  # noqa: E731
+        st = lib.cvs_linear_backward(dy.data_ptr(), s_out, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+                                     z.data_ptr() if keep else None, z.stride(0) if keep else 0, act, 1, m, n, k, p("x", dx), s_dx,
+                                     p("w", dw), s_dx, p("b", db), ws.data_ptr(), ws.numel(), stream())
+        assert st == 0, lib.cvs_last_error()
+        if "x" in wanted:
+            oracle.close(dx, dz @ wd, dz_err @ wd.abs() + (n / 8 + 16) * E * (dz.abs() @ wd.abs()))
+            assert untouched(dxb, dx)
+        if "w" in wanted:
+            oracle.close(dw, dz.T @ xd, dz_err.T @ xd.abs() + (m / 8 + 32) * E * (dz.abs().T @ xd.abs()))
+            assert untouched(dwb, dw)
+        if "b" in wanted:
+            oracle.close(db[:n], dz.sum(0), (dyd.abs() * s_err).sum(0) + (80 + m / 64) * E * dz.abs().sum(0))
+            assert (db[n:] == FILL).all()
+
+
+@pytest.mark.parametrize("rows,d", [(3, 64), (20, 391), (16390, 64), (5, 1032), (2100, 1031)])
+@pytest.mark.parametrize("more,offset", [(8, 0), (8, 8), (5, 1)])
+def test_c_abi_layer_norm_strides(lib, rows, d, more, offset):
+    t = torch.float16
+    _, x = padded(rows, d, d + more, t, offset, randn(rows, d, dtype=t, seed=1))
+    _, dy = padded(rows, d, d + more, t, offset, randn(rows, d, dtype=t, seed=2))
+    ybuf, y = padded(rows, d, d + more, t, offset)
+    dxb, dx = padded(rows, d, d + more, t, offset)
+    mean, rstd = torch.full((rows + 8,), FILL, device="cuda"), torch.full((rows + 8,), FILL, device="cuda")
+    assert lib.cvs_layer_norm(x.data_ptr(), 1, rows, d, d + more, None, None, 1, 1e-5, y.data_ptr(), d + more, mean.data_ptr(),
+                              rstd.data_ptr(), stream()) == 0
+    assert lib.cvs_layer_norm_backward(dy.data_ptr(), d + more, x.data_ptr(), 1, rows, d, d + more, None, 1, mean.data_ptr(),
+                                       rstd.data_ptr(), dx.data_ptr(), d + more, None, None, None, 0, stream()) == 0
+    want, want_dx, *_ = oracle.layer_norm(x, None, None, 1e-5, dy)
+    oracle.close(y, want, 200 * E * (1 + want.abs()))
+    oracle.close(dx, want_dx, 2000 * E * (1 + want.abs()) * dy.double().abs().max())
+    assert untouched(ybuf, y) and untouched(dxb, dx) and (mean[rows:] == FILL).all() and (rstd[rows:] == FILL).all()
