@@ -346,9 +346,10 @@ __global__ void __launch_bounds__(kNormThreads, (backward_blocks<T, CPL>()))
         gr[j] = Cols<VEC>::load(gs, d, tid, kRowThreads, j);
       }
     }
-    // h = x r - mu r. Columns outside the row: dy reads as zero there, so g is zero
-    // and they add nothing to any sum.
-    const Pair r2 = both(rstd), shift = both(-mean * rstd);
+    // h = (x - mu) r, the difference first: x r - mu r would round mu r, which for rows far
+    // from zero is larger than h. Columns outside the row: dy reads as zero there, so g is
+    // zero and they add nothing to any sum.
+    const Pair r2 = both(rstd), shift = both(-mean);
     Pair s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
     for (int j = 0; j < CPL; ++j) {
@@ -359,7 +360,7 @@ __global__ void __launch_bounds__(kNormThreads, (backward_blocks<T, CPL>()))
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const Pair g = pair_at(gr[j], i);
-        const Pair h = pair_fma(pair_at(xr[j], i), r2, shift);
+        const Pair h = pair_mul(pair_add(pair_at(xr[j], i), shift), r2);
         const Pair gw = a.weight ? pair_mul(g, weight_at<kRowThreads>(shared, tid, j, i)) : g;
         s1 = pair_add(s1, gw);
         s2 = pair_fma(gw, h, s2);
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(kNormThreads, (backward_blocks<T, CPL>()))
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const Pair g = pair_at(gr[j], i);
-          const Pair h = pair_fma(pair_at(xr[j], i), r2, shift);
+          const Pair h = pair_mul(pair_add(pair_at(xr[j], i), shift), r2);
           const Pair gw = a.weight ? pair_mul(g, weight_at<kRowThreads>(shared, tid, j, i)) : g;
           set_pair(out, i, pair_mul(r2, pair_add(gw, pair_fma(h, c2, c1))));
         }

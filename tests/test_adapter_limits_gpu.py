@@ -57,6 +57,25 @@ def test_layer_norm_many_wide_rows(cvs, dtype, rows, d):
                randn(d, dtype=t, seed=3), randn(rows, d, dtype=t, seed=4))
 
 
+def test_layer_norm_gradients_of_rows_far_from_zero(cvs):
+    """Rows of 4099 plus whole numbers, whose fp32 mean is exact: the normalised values the
+    backward pass computes again lose nothing to the offset. They are off by the variance's
+    sum (64 terms of one row: half of 64 e at most) and four roundings."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    half = torch.randint(-8, 9, (500, 32), generator=g, device="cuda").float()
+    x = (4099.0 + torch.cat([half, -half], 1)).requires_grad_()
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    dy = x.detach() - 4099.0  # along the rows themselves: the term h mean(g h) is as large as g
+    dx, dw = torch.autograd.grad(cvs.layer_norm(x, w), (x, w), dy)
+    _, want_dx, want_dw, _, (h, rstd, gw) = oracle.layer_norm(x.detach(), w.detach(), None, 1e-5, dy)
+    dh = 36 * E * h.abs()
+    oracle.close(dw, want_dw, (80 + 500 / 64) * E * (dy.double() * h).abs().sum(0) + (dy.double().abs() * dh).sum(0))
+    inner = (gw * h).mean(1, keepdim=True).abs()
+    sums = 40 * E * (gw.abs().mean(1, keepdim=True) + h.abs() * (gw * h).abs().mean(1, keepdim=True))
+    oracle.close(dx, want_dx, rstd * (sums + dh * inner + h.abs() * (gw.abs() * dh).mean(1, keepdim=True)
+                                      + 4 * E * (gw.abs() + h.abs() * inner)) + 36 * E * want_dx.abs())
+
+
 # ---- few tiles: K shared by a cluster ---------------------------------------------------
 @pytest.mark.parametrize("m,k", [(3, 384), (100, 384), (3, 576), (100, 576)])
 def test_linear_clusters_with_ctas_without_a_slice(cvs, m, k):
