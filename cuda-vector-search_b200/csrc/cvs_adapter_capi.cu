@@ -150,12 +150,13 @@ void set_shape(GemmProblem* p, const Tile& t, int64_t m, int64_t n, int64_t k, i
 
 int grid_ctas(const Tile& t, int work, int sms) { return t.cg * std::max(1, std::min(t.slots(sms), work)); }
 
-// Backward: the tile shape, dw's parts along K (= rows), and the workspace.
+// Backward: the tile shape, dw's parts along K (= rows), and the workspace, whose end
+// holds dz (bytes_dz; not needed where the products read dy itself).
 struct BackwardPlan {
   Tile tile;
   int splits;
   int db_parts;
-  size_t dz_offset, db_offset, dw_offset, bytes;
+  size_t dz_offset, db_offset, dw_offset, bytes, bytes_dz;
   int64_t dz_stride;
 };
 
@@ -197,13 +198,13 @@ BackwardPlan plan_backward(int64_t m, int n, int k, int sms) {
   b.db_parts = linear_dz_parts(m, n, sms);
   b.dz_stride = (static_cast<int64_t>(n) + 7) / 8 * 8;
   size_t at = 0;
-  b.dz_offset = at;
-  at += up(static_cast<size_t>(m) * b.dz_stride * 2);
   b.db_offset = at;
   at += up(static_cast<size_t>(b.db_parts) * n * 4);
   b.dw_offset = at;
   if (b.splits > 1) at += up(static_cast<size_t>(p.work) * b.tile.cg * 128 * b.tile.bn * 4);
-  b.bytes = at;
+  b.dz_offset = at;
+  b.bytes_dz = up(static_cast<size_t>(m) * b.dz_stride * 2);
+  b.bytes = at + b.bytes_dz;
   return b;
 }
 
@@ -454,10 +455,11 @@ cvs_status cvs_linear_backward(const void* dy, int64_t dy_stride, const void* x,
   DeviceInfo dev;
   if ((st = device_info(&dev)) != CVS_OK) return st;
   const BackwardPlan plan = plan_backward(m, n, k, dev.sms);
-  if ((st = check_workspace(workspace, workspace_bytes, plan.bytes)) != CVS_OK) return st;
+  const bool dy_tiles = mappable(dy, dy_stride, n);  // TMA can read dy itself
+  const size_t need_bytes = plan.bytes - (act || !dy_tiles ? 0 : plan.bytes_dz);
+  if ((st = check_workspace(workspace, workspace_bytes, need_bytes)) != CVS_OK) return st;
   char* base = static_cast<char*>(workspace);
   const bool bf16 = dtype == CVS_BF16;
-  const bool dy_tiles = aligned16(dy) && dy_stride % 8 == 0 && dy_stride >= n;  // TMA can read dy itself
   Operand dz{dy, dy_stride, false};
   if (act || !dy_tiles) dz = {base + plan.dz_offset, plan.dz_stride, false};
   const bool needs_dz = act || (!dy_tiles && (dx || dw));

@@ -57,12 +57,16 @@ Tensor bytes(size_t n, const Tensor& like) {
 // A 2-D tensor whose rows are contiguous; rows may be any distance apart.
 Tensor with_rows(const Tensor& t) { return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous(); }
 
+// Rows the tensor-memory accelerator can read as they are.
+bool tiles_ok(const Tensor& t) {
+  return reinterpret_cast<std::uintptr_t>(t.data_ptr()) % 16 == 0 && (t.stride(1) == 1 || t.size(1) <= 1) &&
+         (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1)));
+}
+
 // The same with rows the tensor-memory accelerator can read: 16-byte aligned,
 // otherwise copied into rows padded to a multiple of 8 elements.
 Tensor with_tiles(const Tensor& t) {
-  const bool ok = reinterpret_cast<std::uintptr_t>(t.data_ptr()) % 16 == 0 && (t.stride(1) == 1 || t.size(1) <= 1) &&
-                  (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1)));
-  if (ok) return t;
+  if (tiles_ok(t)) return t;
   const Tensor src = with_rows(t);
   const Tensor out = fresh({t.size(0), pad8(t.size(1))}, t.scalar_type(), t);
   check(cvs_align_rows(src.data_ptr(), row_stride(src), code(src), src.size(0), static_cast<int>(src.size(1)), out.data_ptr(),
@@ -281,6 +285,7 @@ class LinearFn : public torch::autograd::Function<LinearFn> {
       const Tensor x = need_w ? with_tiles(saved[0]) : saved[0], w = need_x ? with_tiles(saved[1]) : saved[1];
       size_t need = 0;
       check(cvs_linear_backward_workspace_size(activation, m, static_cast<int>(n), static_cast<int>(k), &need), "linear");
+      if (activation == CVS_ACT_NONE && tiles_ok(dy)) need -= (static_cast<size_t>(m) * pad8(n) * 2 + 255) / 256 * 256;
       const Tensor ws = bytes(need, dy);
       check(cvs_linear_backward(dy.data_ptr(), row_stride(dy), x.data_ptr(), row_stride(x), w.data_ptr(), row_stride(w),
                                 z.defined() ? z.data_ptr() : nullptr, z.defined() ? z.size(1) : 0, activation, code(dy),

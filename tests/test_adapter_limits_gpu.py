@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import adapter_oracle as oracle
-from test_adapter_gpu import DTYPES, E, check_norm, cvs, ids, make_index, randn  # noqa: F401  (cvs: the fixture)
+from test_adapter_gpu import DTYPES, E, check_norm, cvs, ids, make_index, randn, strided  # noqa: F401  (cvs: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -491,3 +491,30 @@ def test_c_abi_layer_norm_strides(lib, rows, d, more, offset):
     oracle.close(y, want, 200 * E * (1 + want.abs()))
     oracle.close(dx, want_dx, 2000 * E * (1 + want.abs()) * dy.double().abs().max())
     assert untouched(ybuf, y) and untouched(dxb, dx) and (mean[rows:] == FILL).all() and (rstd[rows:] == FILL).all()
+
+
+# ---- workspace -------------------------------------------------------------------------
+def test_linear_backward_without_activation_holds_no_copy_of_dy(cvs, lib):
+    m, k, n = 32768, 64, 1536
+    x, w = randn(m, k, dtype=torch.float16, seed=1).requires_grad_(), randn(n, k, dtype=torch.float16, seed=2)
+    dy = randn(m, n, dtype=torch.float16, seed=3)
+    y = cvs.linear(x, w)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    (dx,) = torch.autograd.grad(y, x, dy)
+    held = torch.cuda.max_memory_allocated() - before
+    assert held < dx.nbytes + dy.nbytes // 2  # dx itself, and no m x n halves
+    # The C ABI: less is enough where dy can be read as it is, and refused where not.
+    nbytes, less = size(), m * n * 2
+    assert lib.cvs_linear_backward_workspace_size(0, m, n, k, ctypes.byref(nbytes)) == 0
+    ws = torch.empty(max(nbytes.value - less, 256), dtype=torch.uint8, device="cuda")
+    got = torch.empty_like(dx)
+
+    def call(dy, act=0, z=None):
+        return lib.cvs_linear_backward(dy.data_ptr(), dy.stride(0), x.data_ptr(), k, w.data_ptr(), k, z, n, act, 1, m, n, k,
+                                       got.data_ptr(), k, None, k, None, ws.data_ptr(), nbytes.value - less, stream())
+
+    assert call(dy) == 0 and torch.equal(got, dx)
+    assert call(strided(dy, "odd")) == 3 and b"workspace" in lib.cvs_last_error()
+    assert call(dy, act=2, z=dy.data_ptr()) == 3 and b"workspace" in lib.cvs_last_error()
