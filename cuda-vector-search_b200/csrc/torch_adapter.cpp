@@ -80,9 +80,10 @@ void check_device(const Tensor& t, const char* name, const Tensor& first) {
   TORCH_CHECK(t.device() == first.device(), name, " must be on the same device as the input");
 }
 
-// A leaf whose gradient accumulator was made on another stream (by a graph that is
-// still alive) would make a captured backward pass wait for that stream, which ends
-// the capture and, from the autograd thread, the process. Refused before that.
+// A leaf whose gradient accumulator was made on the default stream (by a graph that is
+// still alive) would make a captured backward pass wait for that stream, which cannot take
+// part in a capture: that ends it and, from the autograd thread, the process. Refused
+// before that. (Another stream's accumulator, a warm-up's, joins the capture.)
 void check_capture(std::initializer_list<const Tensor*> inputs) {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   if (!at::GradMode::is_enabled()) return;
@@ -91,9 +92,9 @@ void check_capture(std::initializer_list<const Tensor*> inputs) {
     const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
     if (!node) continue;
     const auto stream = node->stream();
-    TORCH_CHECK(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(t->device().index()).unwrap(),
-                "a parameter of a captured backward pass still belongs to an autograd graph made on another stream; "
-                "release that graph's outputs before the capture, or run it on the capture's stream");
+    TORCH_CHECK(!stream.has_value() || *stream != c10::cuda::getDefaultCUDAStream(t->device().index()).unwrap(),
+                "a parameter of a captured backward pass still belongs to an autograd graph made on another stream, "
+                "the default one; release that graph's outputs before the capture, or run it on another stream");
   }
 }
 

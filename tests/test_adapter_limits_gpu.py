@@ -518,3 +518,41 @@ def test_linear_backward_without_activation_holds_no_copy_of_dy(cvs, lib):
     assert call(dy) == 0 and torch.equal(got, dx)
     assert call(strided(dy, "odd")) == 3 and b"workspace" in lib.cvs_last_error()
     assert call(dy, act=2, z=dy.data_ptr()) == 3 and b"workspace" in lib.cvs_last_error()
+
+
+# ---- graphs --------------------------------------------------------------------------------
+def test_capture_after_a_warm_up_on_another_stream():
+    """torch's own recipe in a process of its own: training steps on a side stream whose last
+    loss stays alive, then the step captured on the capture's stream; the replay's gradients
+    are the warm-up's."""
+    code = """
+import torch, cuda_vector_search as cvs
+torch.manual_seed(0)
+index = cvs.Index(torch.randn(2000, 128, device="cuda"))
+adapter = cvs.Adapter(128, device="cuda")
+q = torch.randn(64, 128, device="cuda", dtype=torch.float16)
+c, r = torch.randint(2000, (64,), device="cuda"), torch.randint(2000, (64, 4), device="cuda")
+def step():
+    adapter.zero_grad(set_to_none=True)
+    loss = index.preference_loss(adapter(q), c, r, reference=q)
+    loss.backward()
+    return loss
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(side):
+    for _ in range(3):
+        loss = step()
+torch.cuda.current_stream().wait_stream(side)
+want = [p.grad.clone() for p in adapter.parameters()]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = step()
+for _ in range(3):
+    for p in adapter.parameters():
+        p.grad.fill_(7.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(captured, loss) and all(torch.equal(p.grad, w) for p, w in zip(adapter.parameters(), want))
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=LIB.parent.parent, capture_output=True, text=True, timeout=200)
+    assert run.returncode == 0, run.stderr[-2000:]
