@@ -556,3 +556,39 @@ for _ in range(3):
 """
     run = subprocess.run([sys.executable, "-c", code], cwd=LIB.parent.parent, capture_output=True, text=True, timeout=200)
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+# ---- broadcast inputs ------------------------------------------------------------------
+def test_preference_of_one_query_and_shared_rejected_rows(cvs):
+    """One query expanded over several chosen rows, one list of rejected rows for all of them:
+    the values of the copies, and the query's gradient summed over its uses."""
+    index = make_index(cvs, 300, 96, "cosine")
+    q = randn(1, 96, dtype=torch.float32, seed=1).requires_grad_()
+    ref, c, rej = randn(1, 96, dtype=torch.float32, seed=2), ids(300, 20, seed=3, gone=0.1), ids(300, 1, 5, seed=4, gone=0.1)
+    loss, m = index.preference_loss(q.expand(20, 96), c, rej.expand(20, 5), reference=ref.expand(20, 96), return_margins=True)
+    (dq,) = torch.autograd.grad(loss, q)
+    dense = q.detach().expand(20, 96).contiguous().requires_grad_()
+    loss2, m2 = index.preference_loss(dense, c, rej.expand(20, 5).contiguous(), reference=ref.expand(20, 96).contiguous(),
+                                      return_margins=True)
+    (each,) = torch.autograd.grad(loss2, dense)
+    assert torch.equal(loss, loss2) and torch.equal(m, m2)
+    oracle.close(dq[0], each.double().sum(0), 20 * E * each.double().abs().sum(0))
+
+
+def test_adapter_of_more_dimensions(cvs):
+    """[2, 3, d] in, the same rows as [6, d], gradients included; a batch without rows."""
+    torch.manual_seed(0)
+    a = cvs.Adapter(64, activation="silu", device="cuda")
+    with torch.no_grad():
+        a.weight2.copy_(torch.randn(64, 128) * 0.1)
+    x = randn(2, 3, 64, dtype=torch.float16, seed=1).requires_grad_()
+    flat = x.detach().reshape(6, 64).requires_grad_()
+    y, want = a(x), a(flat)
+    assert y.shape == x.shape and torch.equal(y.reshape(6, 64), want)
+    dy = randn(2, 3, 64, dtype=torch.float16, seed=2)
+    got = torch.autograd.grad(y, (x, *a.parameters()), dy)
+    exp = torch.autograd.grad(want, (flat, *a.parameters()), dy.reshape(6, 64))
+    assert all(torch.equal(g.reshape(e.shape), e) for g, e in zip(got, exp))
+    none = randn(0, 64, dtype=torch.float16, seed=1).requires_grad_()
+    dx, *grads = torch.autograd.grad(a(none), (none, *a.parameters()), torch.empty(0, 64, dtype=torch.float16, device="cuda"))
+    assert dx.shape == (0, 64) and all((g == 0).all() for g in grads)
