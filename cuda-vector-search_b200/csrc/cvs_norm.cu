@@ -13,7 +13,7 @@
 //
 // A row belongs to one warp (width up to 1024: no barrier) or to one block of 8 warps
 // (up to 8192). Aligned rows of one warp come as bulk copies into a ring per warp in
-// shared memory (forward: from 16384 rows on), so that the bytes in flight cost no
+// shared memory (forward: half-precision, from 2^23 elements on), so that the bytes in flight cost no
 // registers and each SM's warps never wait for one another's rows. In the backward pass
 // every thread keeps the sums of dw and db for the columns it owns while its warp walks
 // the rows, so the weights' gradients cost no traffic per row; the blocks' sums go to the
@@ -473,8 +473,16 @@ unsigned norm_grid(long long rows, int rows_per_block, int blocks) {
 }
 
 
-// Whether forward blocks walk several rounds of rows.
-bool norm_staged(long long rows, int d) { return rows >= (row_warps(d) == 1 ? 16384 : 2048); }
+// Whether forward blocks walk several rounds of rows with the weights (and, aligned rows of
+// one warp, the rows) staged in shared memory. That pays once a half-precision matrix is
+// large against one round of blocks. Straight / staged, us, fp16: 768 columns, 4096 rows 5.3
+// / 5.8, 16384 16.3 / 12.8, 131072 99 / 78; 256 columns, 16384 6.9 / 7.2, 32768 11.8 / 11.4;
+// 64 columns, 131072 38.1 / 39.0; 1001 (unaligned), 16384 24.8 / 25.5, 131072 161 / 156; one
+// row a block, 2048 columns, 2048 rows 8.0 / 8.6, 4096 14.2 / 12.9, 16384 50 / 40; 8192
+// columns, 4096 rows 34.5 / 35.4, 16384 115 / 113. A staged fp32 row is twice as long and its
+// ring half as deep: 768 columns, 16384 rows 20.7 / 20.2, 65536 67 / 76, 131072 127 / 149;
+// 8192 columns, 16384 rows 179 / 185.
+bool norm_staged(long long rows, int d) { return row_warps(d) == 1 ? rows * d >= (1 << 23) : rows >= 4096; }
 
 // Blocks of `kern` an SM holds at once.
 template <class K>
@@ -487,25 +495,28 @@ template <class T, bool VEC, int WARPS, int CPL>
 cudaError_t launch_one(NormArgs a, bool backward, int num_sms, cudaStream_t stream) {
   constexpr int kPerBlock = kNormWarps / WARPS;
   const size_t weights = static_cast<size_t>(CPL) * 4 * 32 * WARPS * sizeof(float2);
-  if (a.stall && !(norm_ring<VEC, WARPS>() && (backward || norm_staged(a.rows, a.d)))) return cudaErrorNotSupported;
+  constexpr bool kHalf = sizeof(T) == 2;
+  if (a.stall && !(norm_ring<VEC, WARPS>() && (backward || (kHalf && norm_staged(a.rows, a.d))))) return cudaErrorNotSupported;
   if (!backward) {
-    if (norm_staged(a.rows, a.d)) {
-      // One round of blocks: each SM's share of the rows is the same.
-      auto kern = norm_forward_kernel<T, VEC, WARPS, CPL, true>;
-      size_t smem = 2 * weights;
-      int per_warp = 1;  // rows a warp has at work
-      if (norm_ring<VEC, WARPS>()) {
-        const size_t per = static_cast<size_t>(kNormWarps) * a.d * sizeof(T);
-        a.slots = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kForwardSlots, (kForwardShared - smem) / per)));
-        smem += a.slots * per;
-      } else if (WARPS == 1) {
-        per_warp = kForwardRows;
+    if constexpr (kHalf) {
+      if (norm_staged(a.rows, a.d)) {
+        // One round of blocks: each SM's share of the rows is the same.
+        auto kern = norm_forward_kernel<T, VEC, WARPS, CPL, true>;
+        size_t smem = 2 * weights;
+        int per_warp = 1;  // rows a warp has at work
+        if (norm_ring<VEC, WARPS>()) {
+          const size_t per = static_cast<size_t>(kNormWarps) * a.d * sizeof(T);
+          a.slots = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kForwardSlots, (kForwardShared - smem) / per)));
+          smem += a.slots * per;
+        } else if (WARPS == 1) {
+          per_warp = kForwardRows;
+        }
+        static std::atomic<unsigned long long> allowed{0};
+        const cudaError_t e = allow_smem(kern, kForwardShared, allowed);
+        if (e != cudaSuccess) return e;
+        const unsigned grid = norm_grid(a.rows, kPerBlock * per_warp, blocks_per_sm(kern, smem) * num_sms);
+        return launch_programmatic(kern, dim3(grid), dim3(kNormThreads), smem, stream, a);
       }
-      static std::atomic<unsigned long long> allowed{0};
-      const cudaError_t e = allow_smem(kern, kForwardShared, allowed);
-      if (e != cudaSuccess) return e;
-      const unsigned grid = norm_grid(a.rows, kPerBlock * per_warp, blocks_per_sm(kern, smem) * num_sms);
-      return launch_programmatic(kern, dim3(grid), dim3(kNormThreads), smem, stream, a);
     }
     const unsigned grid = norm_grid(a.rows, WARPS == 1 ? kPerBlock * kForwardRows : 1, INT_MAX);
     return launch_programmatic(norm_forward_kernel<T, VEC, WARPS, CPL, false>, dim3(grid), dim3(kNormThreads), 0, stream, a);
