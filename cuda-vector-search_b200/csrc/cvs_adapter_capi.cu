@@ -103,8 +103,12 @@ constexpr Tile kTiles[3] = {{2, 256}, {1, 128}, {1, 64}};
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Time of one work item in units of 128 x 64 x 64 products per SM: larger tiles
-// keep the tensor cores busier per byte of shared memory read.
+// Time of one round of work items, in units of half the smallest tile's: larger tiles keep the
+// tensor cores busier per byte of shared memory read. Measured (us, tiles of 256 x 256 by a CTA
+// pair / 128 x 128 / 128 x 64, K = 768, rounds in brackets): 18944 x 128 10.8 [1] / 8.4 [1] /
+// 10.1 [2]; 18944 x 256 12.0 [1] / 12.4 [2] / 16.0 [4]; 4096 x 768 10.4 [1] / 11.2 [2] / 13.7
+// [3]; 16384 x 768 23.5 [3] / 30.3 [6] / 42.1 [11]; 131072 x 768 131 [21] / 221 [42] / 349
+// [84]: 6.2 : 4.2-5.3 : 3.4-4.2 us a round in the larger ones.
 double tile_cost(const Tile& t) { return t.cg == 2 ? 4.0 : (t.bn == 128 ? 2.7 : 2.0); }
 
 // The tile shape whose rounds of work items over the SMs take least: large tiles
@@ -333,11 +337,14 @@ cvs_status cvs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_
   DeviceInfo dev;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  // Up to two rows the CUDA cores stream the weights fastest (768 -> 1536, one, two, four,
-  // eight rows: 2.4, 3.3, 5.0, 8.6 us, against 5.0 us on the tensor cores at each); rows
-  // of any alignment stay there a little longer rather than have the weights copied.
+  // One row, and two of up to 2048 columns, the CUDA cores take fastest, streaming the weights.
+  // Rows 1 / 2 / 3 on CUDA cores against any of them on the tensor cores, us: 256 -> 256 1.6 /
+  // 1.9 / 2.3, 4.3; 768 -> 1536 2.1 / 3.0 / 3.8, 4.8; 1024 -> 16384 8.4 / 11.4 / 15.2, 12.6;
+  // 2048 -> 2048 2.6 / 5.2 / 7.2, 6.1; 2048 -> 8192 8.8 / 10.9 / 14.9, 13.2; 4096 -> 1024 3.3 /
+  // 8.6 / 12.3, 7.2; 4096 -> 4096 8.0 / 17.7 / 24.4, 12.8. Rows of any alignment stay there up
+  // to kLinearSmallRows rather than have the weights copied.
   const bool tiles = mappable(x, m > 1 ? x_stride : ceil_div(k, 8) * 8, k) && mappable(w, w_stride, k);
-  if (m <= 2 || (m <= kLinearSmallRows && !tiles)) {
+  if (m == 1 || (m == 2 && k <= 2048) || (m <= kLinearSmallRows && !tiles)) {
     if ((m > 1 && x_stride < 0) || w_stride < k)
       return fail(CVS_ERR_INVALID_ARGUMENT, "bad row stride");
     if ((st = device_info(&dev)) != CVS_OK) return st;

@@ -247,7 +247,7 @@ cudaError_t norm_launch(const NormArgs& a, int dtype, bool backward, int num_sms
 
 // ---- linear layer -------------------------------------------------------------
 enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
-constexpr int kLinearSmallRows = 8;  // rows up to which the weights are streamed by CUDA cores
+constexpr int kLinearSmallRows = 8;  // rows of any alignment up to which CUDA cores stream the weights
 
 // One product out[m][n] = A B^T over kblocks slices of 64 along K, cut into
 // `splits` parts of kper slices. All pointers hold halves of the call's type

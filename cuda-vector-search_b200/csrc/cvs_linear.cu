@@ -12,7 +12,7 @@
 //
 // Bound: 2 m n k operations at the tensor cores' rate for batches of thousands of rows;
 // below that latency and the weights' bytes, where split_kernel shares K among a cluster
-// and linear_small_kernel (one or two rows) streams the weights once with CUDA cores.
+// and linear_small_kernel (one row, two narrow ones) streams the weights once with CUDA cores.
 // Measured: 131072 x 1536 -> 768 bf16 with bias 220 us (1.41 PF/s), with residual 232 us;
 // 16384 x 768 -> 1536 with bias 33 us, forward for training with GELU 44 us, backward 96
 // us; 256 x 768 -> 1536 GELU 7.1 us; one row 2.5 us.

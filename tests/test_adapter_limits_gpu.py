@@ -102,6 +102,16 @@ def test_linear_clusters_with_ctas_without_a_slice(cvs, m, k):
     assert all(torch.equal(cvs.linear(x, w), first) for _ in range(200))
 
 
+@pytest.mark.parametrize("k", [2048, 2056, 4096, 2050])
+@pytest.mark.parametrize("m", [1, 2])
+def test_linear_of_one_and_two_wide_rows(cvs, m, k):
+    """Either side of the width where two rows leave the CUDA cores; 2050: unaligned rows stay."""
+    t = torch.bfloat16
+    x, w, b = randn(m, k, dtype=t, seed=1), randn(100, k, dtype=t, seed=2, scale=k**-0.5), randn(100, dtype=t, seed=3)
+    want, z, _, scale = oracle.linear(x, w, b, "silu", None)
+    oracle.close(cvs.linear(x, w, b, activation="silu"), want, 1.13 * (k / 8 + 16) * E * scale + 16 * E * z.abs())
+
+
 # ---- two host threads ---------------------------------------------------------------
 def in_threads(*calls, repeats=4000):
     """Each call over and over in a host thread of its own (foreign calls release the
