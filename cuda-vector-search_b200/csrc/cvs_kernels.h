@@ -21,7 +21,8 @@ constexpr int kTcK = 64;           // halves per K slice (one 128-byte swizzled 
 // histograms and compaction buffers holds, at most this many (the barrier
 // arrays are sized for it).
 constexpr int kTcMaxStages = 8;
-constexpr int kSmemBudget = 232448 - 1024;  // dynamic shared memory per CTA, less the alignment slack
+constexpr int kSmemLimit = 232448;          // dynamic shared memory per CTA
+constexpr int kSmemBudget = kSmemLimit - 1024;  // less the alignment slack
 constexpr int kTcMaxResidentSlices = 7;  // queries stay in smem when d_pad <= 448
 // Dry tiles of the top-k epilogues (see cvs_epilogue.cuh): at most this many
 // (TileSource in cvs_sched.cuh keeps two).

@@ -414,8 +414,8 @@ cudaError_t merge_keys_launch(const MergeKeysArgs& a, cudaStream_t stream) {
   // Lists without counts must be packed (the filter walks them as one run).
   if (!a.counts && a.per_list != a.stride) return cudaErrorInvalidValue;
   const size_t smem = keys_smem(a.k);
-  cudaError_t e = cudaFuncSetAttribute(merge_keys_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_smem(merge_keys_kernel, static_cast<int>(keys_smem(kMergeMaxK)), allowed);
   if (e != cudaSuccess) return e;
   // Programmatic dependent launch: the merge grid may be scheduled while the
   // search kernel's last CTAs finish (it waits for their results on the device).
@@ -439,9 +439,8 @@ cudaError_t prepare_launch(void* p, size_t bytes, const void* q_src, void* q_dst
 cudaError_t merge_lists_launch(const MergeListsArgs& a, cudaStream_t stream) {
   if (a.k < 1 || a.k > kMergeMaxK || a.b < 1) return cudaErrorInvalidValue;
   const size_t smem = merge_smem(a.k);
-  cudaError_t e = cudaFuncSetAttribute(merge_lists_kernel,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_smem(merge_lists_kernel, static_cast<int>(merge_smem(kMergeMaxK)), allowed);
   if (e != cudaSuccess) return e;
   const unsigned grid = static_cast<unsigned>((a.b + kMergeWarps - 1) / kMergeWarps);
   merge_lists_kernel<<<grid, kMergeWarps * 32, smem, stream>>>(a);

@@ -412,8 +412,8 @@ cudaError_t pair_launch_one(const CUtensorMap* qmap, const CUtensorMap* xmap, co
   const PairLayout l = pair_layout(QRES, a.ksl, Epi::kSubs, Epi::kScratchKeys);
   const size_t smem = static_cast<size_t>(l.total) + 1024;
   auto kern = tc_pair_kernel<QRES, Epi>;
-  cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_smem(kern, kSmemLimit, allowed);
   if (e != cudaSuccess) return e;
   const unsigned grid = 2u * static_cast<unsigned>(a.qtiles) * static_cast<unsigned>(a.segs);
   return launch_programmatic(kern, dim3(grid), dim3(pair_threads(Epi::kSubs)), smem, stream, *qmap, *xmap, a);
@@ -424,9 +424,8 @@ int pair_clusters_one(int ksl) {
   const PairLayout l = pair_layout(QRES, ksl, Epi::kSubs, Epi::kScratchKeys);
   const size_t smem = static_cast<size_t>(l.total) + 1024;
   auto kern = tc_pair_kernel<QRES, Epi>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) !=
-      cudaSuccess)
-    return 0;
+  static std::atomic<unsigned long long> allowed{0};
+  if (allow_smem(kern, kSmemLimit, allowed) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2, 1, 1);
   cfg.blockDim = dim3(pair_threads(Epi::kSubs), 1, 1);

@@ -383,8 +383,8 @@ cudaError_t launch_one(const CUtensorMap* qmap, const CUtensorMap* xmap, const T
   const Layout l = make_layout(QRES, a.ksl, Epi::kSubs, Epi::kScratchKeys);
   const size_t smem = static_cast<size_t>(l.total) + 1024;
   auto kern = tc_search_kernel<QRES, Epi>;
-  cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_smem(kern, kSmemLimit, allowed);
   if (e != cudaSuccess) return e;
   const unsigned grid = static_cast<unsigned>(a.qtiles) * static_cast<unsigned>(a.segs);
   return launch_programmatic(kern, dim3(grid), dim3(tc_threads(Epi::kSubs)), smem, stream, *qmap, *xmap, a);
