@@ -13,9 +13,10 @@
 // Bound: 2 m n k operations at the tensor cores' rate for batches of thousands of rows;
 // below that latency and the weights' bytes, where split_kernel shares K among a cluster
 // and linear_small_kernel (one row, two narrow ones) streams the weights once with CUDA cores.
-// Measured: 131072 x 1536 -> 768 bf16 with bias 220 us (1.41 PF/s), with residual 232 us;
-// 16384 x 768 -> 1536 with bias 33 us, forward for training with GELU 44 us, backward 96
-// us; 256 x 768 -> 1536 GELU 7.1 us; one row 2.5 us.
+// Measured: 131072 x 1536 -> 768 bf16 with bias 234-240 us at an SM clock of 1965 MHz (1.3
+// PF/s), with residual 253-260 us; in runs of about a second, which the power cap holds near
+// 1050 MHz, 274 and 299 us. 16384 x 768 -> 1536 with bias 33 us, forward for training with
+// GELU 44 us, backward 96 us; 256 x 768 -> 1536 GELU 7.1 us; one row 2.5 us.
 //
 // The pre-activation z is kept for the backward pass as fp16, also for bf16 rows:
 // the activations' derivatives are constant where fp16 ends (|z| > 65504), and

@@ -18,9 +18,9 @@
 // every thread keeps the sums of dw and db for the columns it owns while its warp walks
 // the rows, so the weights' gradients cost no traffic per row; the blocks' sums go to the
 // workspace and a second small kernel adds them in a fixed order, which makes the result
-// the same on every run. Measured: 262144 x 768 fp16 forward 140 us (5.8 TB/s), backward
-// 204 us (5.9 TB/s); with rows loaded into registers 157 and 372 us. 16384 x 768 bf16: 14
-// and 23 us, of which about half is the kernels' start and end.
+// the same on every run. Measured: 262144 x 768 fp16 forward 140-150 us (5.4-5.8 TB/s),
+// backward 192 us (6.3 TB/s); with rows loaded into registers 157 and 372 us. 16384 x 768
+// bf16: 12 and 20 us, of which about half is the kernels' start and end.
 #include "cvs_device.cuh"
 #include "cvs_elem.cuh"
 #include "cvs_kernels.h"
