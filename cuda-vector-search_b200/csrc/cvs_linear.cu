@@ -22,7 +22,9 @@
 // the activations' derivatives are constant where fp16 ends (|z| > 65504), and
 // fp16's 11 bits keep the derivative's error an order below bf16's own rounding.
 // dz is rounded once to the rows' type, because both products that read it take
-// half-precision operands.
+// half-precision operands. That puts dx and dw 2.3e-3 (bf16; fp16 3.0e-4) of their norm from
+// float64, where one rounding of the exact gradient is 1.7e-3 (2.1e-4) away; carrying dz's
+// remainder as a second operand would double the products. dbias sums the unrounded dz.
 #include "cvs_gemm.cuh"
 
 namespace cvs {

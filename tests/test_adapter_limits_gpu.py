@@ -1,6 +1,7 @@
 """The adapter's operators where a first set of sizes did not look."""
 
 import ctypes
+import os
 import subprocess
 import sys
 import threading
@@ -11,6 +12,7 @@ import torch
 
 import adapter_oracle as oracle
 from test_adapter_gpu import DTYPES, E, check_norm, cvs, ids, make_index, randn, strided  # noqa: F401  (cvs: the fixture)
+from test_sharded_gloo import _free_port
 
 pytestmark = pytest.mark.gpu
 
@@ -361,7 +363,7 @@ def test_counts_past_32_bits_are_refused(cvs):
 
 # ---- training as documented ------------------------------------------------------------
 def test_the_documented_training_loop(cvs):
-    """README's loop as it stands: the fp32 copies take every step, the parameters are their
+    """The documented loop as it stands: the fp32 copies take every step, the parameters are their
     rounded values, and the gradient the loop ends on is the adapter's own."""
     text = (LIB.parent.parent.parent / "README.md").read_text()
     code = text[text.index("from cuda_vector_search import Adapter, Index") :]
@@ -614,3 +616,26 @@ def test_adapter_of_more_dimensions(cvs):
     none = randn(0, 64, dtype=torch.float16, seed=1).requires_grad_()
     dx, *grads = torch.autograd.grad(a(none), (none, *a.parameters()), torch.empty(0, 64, dtype=torch.float16, device="cuda"))
     assert dx.shape == (0, 64) and all((g == 0).all() for g in grads)
+
+
+def test_adapter_in_a_sharded_search():
+    """The real adapter in front of a sharded index of one rank: the plain index's results."""
+    code = """
+import os, torch, torch.distributed as dist
+from datetime import timedelta
+import cuda_vector_search as cvs
+dist.init_process_group("nccl", rank=0, world_size=1, timeout=timedelta(seconds=60), device_id=torch.device("cuda", 0))
+torch.manual_seed(0)
+x, q = torch.randn(3000, 96), torch.randn(20, 96)
+a = cvs.Adapter(96, device="cuda")
+with torch.no_grad():
+    a.weight2.copy_(torch.randn(96, 192) * 0.1)
+v, i = cvs.ShardedIndex(x.numpy()).search(q.numpy(), 5, adapter=a)
+v2, i2 = cvs.Index(x).search(q.cuda(), 5, adapter=a)
+assert torch.equal(v, v2) and torch.equal(i, i2) and not v.requires_grad
+torch.cuda.synchronize()
+dist.destroy_process_group()
+"""
+    env = dict(os.environ, MASTER_ADDR="127.0.0.1", MASTER_PORT=str(_free_port()), NCCL_SOCKET_IFNAME="lo")
+    run = subprocess.run([sys.executable, "-c", code], cwd=LIB.parent.parent, capture_output=True, text=True, timeout=200, env=env)
+    assert run.returncode == 0, run.stderr[-2000:]
