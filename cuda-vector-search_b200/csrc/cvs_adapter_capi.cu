@@ -38,7 +38,7 @@ cvs_status run_norm(NormArgs& a, int dtype, bool backward, const DeviceInfo& dev
   g_norm_stall = 0;  // one call only
   const cudaError_t e = norm_launch(a, dtype, backward, dev.sms, s);
   if (a.stall && e == cudaErrorNotSupported)
-    return fail(CVS_ERR_INVALID_ARGUMENT, "the stall test hook needs aligned rows of up to 1024 columns (forward: halves, at least 2^23 of them)");
+    return fail(CVS_ERR_INVALID_ARGUMENT, "the stall test hook needs aligned rows of up to 1024 columns (forward: halves, more than 2^22 of them)");
   return e == cudaSuccess ? CVS_OK : cuda_fail(e, backward ? "layer norm backward launch" : "layer norm launch");
 }
 

@@ -13,7 +13,7 @@
 //
 // A row belongs to one warp (width up to 1024: no barrier) or to one block of 8 warps
 // (up to 8192). Aligned rows of one warp come as bulk copies into a ring per warp in
-// shared memory (forward: half-precision, from 2^23 elements on), so that the bytes in flight cost no
+// shared memory (forward: in large matrices, norm_staged), so that the bytes in flight cost no
 // registers and each SM's warps never wait for one another's rows. In the backward pass
 // every thread keeps the sums of dw and db for the columns it owns while its warp walks
 // the rows, so the weights' gradients cost no traffic per row; the blocks' sums go to the
@@ -474,15 +474,29 @@ unsigned norm_grid(long long rows, int rows_per_block, int blocks) {
 
 
 // Whether forward blocks walk several rounds of rows with the weights (and, aligned rows of
-// one warp, the rows) staged in shared memory. That pays once a half-precision matrix is
-// large against one round of blocks. Straight / staged, us, fp16: 768 columns, 4096 rows 5.3
-// / 5.8, 16384 16.3 / 12.8, 131072 99 / 78; 256 columns, 16384 6.9 / 7.2, 32768 11.8 / 11.4;
-// 64 columns, 131072 38.1 / 39.0; 1001 (unaligned), 16384 24.8 / 25.5, 131072 161 / 156; one
-// row a block, 2048 columns, 2048 rows 8.0 / 8.6, 4096 14.2 / 12.9, 16384 50 / 40; 8192
-// columns, 4096 rows 34.5 / 35.4, 16384 115 / 113. A staged fp32 row is twice as long and its
-// ring half as deep: 768 columns, 16384 rows 20.7 / 20.2, 65536 67 / 76, 131072 127 / 149;
-// 8192 columns, 16384 rows 179 / 185.
-bool norm_staged(long long rows, int d) { return row_warps(d) == 1 ? rows * d >= (1 << 23) : rows >= 4096; }
+// one warp, the rows) staged in shared memory: where the matrix is large against one round
+// of blocks. Straight / staged, us:
+//   fp16, one warp a row: 64 columns, 65536 rows 20.1 / 21.0; 256 columns, 16384 rows 6.9 /
+//     7.2, 131072 39.2 / 38.6; 400 columns, 16384 rows 10.8 / 9.2, 131072 61 / 51; 768
+//     columns, 4096 rows 5.3 / 5.8, 16384 16.3 / 12.8, 131072 99 / 78; unaligned: 391 columns,
+//     16384 rows 13.7 / 12.9, 131072 87 / 69; 767 columns, 131072 rows 120 / 127.
+//   fp16, a block a row: 2048 columns, 2048 rows 8.0 / 8.6, 4096 14.2 / 12.9, 16384 50 / 40;
+//     8192 columns, 4096 rows 34.5 / 35.4, 16384 115 / 113.
+//   fp32, one warp a row (whose ring is half as deep): 512 columns, 16384 rows 14.3 / 15.0,
+//     131072 83 / 102; 768 columns, 16384 rows 20.6 / 20.3, 131072 127 / 149; 1000 columns,
+//     4096 rows 9.4 / 9.4, 16384 30 / 26, 32768 53 / 52, 131072 186 / 199; unaligned: 511
+//     columns, 131072 rows 86 / 93; 1001 columns, 131072 rows 182 / 175.
+//   fp32, a block a row: 1031 columns, 8192 rows 26 / 22, 65536 194 / 153; 2048 columns, 4096
+//     rows 16.4 / 18.1, 8192 30.1 / 30.5, 32768 110 / 101; 8192 columns, 16384 rows 179 / 185.
+template <class T, bool VEC, int WARPS, int CPL>
+constexpr bool may_stage() { return sizeof(T) == 2 || WARPS > 1 || CPL > 3; }
+template <class T, bool VEC, int WARPS, int CPL>
+bool norm_staged(long long rows, int d) {
+  constexpr bool kHalf = sizeof(T) == 2;
+  if (WARPS > 1) return rows >= (kHalf ? 4096 : 8192);
+  const long long cells = rows * d;
+  return may_stage<T, VEC, WARPS, CPL>() && cells > (1 << 22) && (kHalf || !VEC || cells <= (1 << 25));
+}
 
 // Blocks of `kern` an SM holds at once.
 template <class K>
@@ -495,11 +509,11 @@ template <class T, bool VEC, int WARPS, int CPL>
 cudaError_t launch_one(NormArgs a, bool backward, int num_sms, cudaStream_t stream) {
   constexpr int kPerBlock = kNormWarps / WARPS;
   const size_t weights = static_cast<size_t>(CPL) * 4 * 32 * WARPS * sizeof(float2);
-  constexpr bool kHalf = sizeof(T) == 2;
-  if (a.stall && !(norm_ring<VEC, WARPS>() && (backward || (kHalf && norm_staged(a.rows, a.d))))) return cudaErrorNotSupported;
+  const bool stage = norm_staged<T, VEC, WARPS, CPL>(a.rows, a.d);
+  if (a.stall && !(norm_ring<VEC, WARPS>() && (backward || stage))) return cudaErrorNotSupported;
   if (!backward) {
-    if constexpr (kHalf) {
-      if (norm_staged(a.rows, a.d)) {
+    if constexpr (may_stage<T, VEC, WARPS, CPL>()) {
+      if (stage) {
         // One round of blocks: each SM's share of the rows is the same.
         auto kern = norm_forward_kernel<T, VEC, WARPS, CPL, true>;
         size_t smem = 2 * weights;

@@ -241,7 +241,7 @@ cvs_status cvs_layer_norm_backward(const void* dy, int64_t dy_stride, const void
  * cvs_layer_norm or cvs_layer_norm_backward call with rows to work on, made on this
  * host thread, copies none of them, and its waits give up after wait_cycles SM clocks
  * (1000 .. 2^40). Calls whose kernel has no such wait (rows that are unaligned or wider
- * than 1024; forward: fp32, or fewer than 2^23 elements) disarm it and return
+ * than 1024; forward: also small matrices, and fp32 ones) disarm it and return
  * CVS_ERR_INVALID_ARGUMENT. The armed call's results are undefined.
  */
 cvs_status cvs_debug_stall_next_norm(int64_t wait_cycles);

@@ -52,18 +52,19 @@ def test_layer_norm_widths_that_end_before_the_last_group(cvs, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,d", [(2048, 4104), (2500, 8191), (2500, 8192), (4096, 4104), (4100, 8191)])
+@pytest.mark.parametrize("rows,d", [(2048, 4104), (2500, 8191), (2500, 8192), (4096, 4104), (4100, 8191), (8200, 4104)])
 def test_layer_norm_many_wide_rows(cvs, dtype, rows, d):
     t = DTYPES[dtype]
     check_norm(cvs, randn(rows, d, dtype=t, seed=1, shift=0.5), randn(d, dtype=t, seed=2, shift=1.0),
                randn(d, dtype=t, seed=3), randn(rows, d, dtype=t, seed=4))
 
 
-@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
-@pytest.mark.parametrize("rows,d", [(1 << 20, 8), ((1 << 20) + 9, 8), (88000, 96), (140000, 60), (8200, 1024), (4100, 2048)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,d", [(1 << 20, 8), ((1 << 20) + 9, 8), (88000, 96), (140000, 60), (8200, 1024), (4200, 1001),
+                                    (33000, 1024), (4100, 2048), (8200, 1032), (8200, 1031)])
 def test_layer_norm_many_elements(cvs, dtype, rows, d):
-    """2^23 elements (4096 rows of a block each) and more: the forward kernels that stage the
-    weights and, aligned, the rows; the same bits as the first rows alone, which are too few."""
+    """Enough elements for the forward kernels that stage the weights and, aligned, the rows
+    (types and widths differ in how many that is): the same bits as a few rows alone."""
     t = DTYPES[dtype]
     x, w, b = randn(rows, d, dtype=t, seed=1, scale=2.0, shift=0.5), randn(d, dtype=t, seed=2, shift=1.0), randn(d, dtype=t, seed=3)
     y = cvs.layer_norm(x, w, b)
