@@ -30,6 +30,9 @@ def lib():
     lib.cvs_linear_backward_workspace_size.argtypes = [i32, i64, i32, i32, ctypes.POINTER(size)]
     lib.cvs_linear_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i64, i32, i32, vp, i64, vp, i64, vp, vp,
                                         size, vp]
+    lib.cvs_preference_loss_workspace_size.argtypes = [i64, i32, ctypes.POINTER(size)]
+    lib.cvs_preference_grad.argtypes = [vp, i64, i64, i32, vp, vp, i32, vp, vp]
+    lib.cvs_align_rows.argtypes = [vp, i64, i32, i64, i32, vp, i64, vp]
     lib.cvs_debug_stall_next_norm.argtypes = [i64]
     lib.cvs_poll_device_error.argtypes = [i32, ctypes.POINTER(ctypes.c_int)]
     lib.cvs_preference_loss.argtypes = [vp, i32, i64, vp, i32, i64, i64, i32, i32, vp, i64, i32, vp, vp, i64, i32, f32, f32,
@@ -640,3 +643,52 @@ dist.destroy_process_group()
     env = dict(os.environ, MASTER_ADDR="127.0.0.1", MASTER_PORT=str(_free_port()), NCCL_SOCKET_IFNAME="lo")
     run = subprocess.run([sys.executable, "-c", code], cwd=LIB.parent.parent, capture_output=True, text=True, timeout=200, env=env)
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("more,offset", [(8, 0), (5, 1)])
+@pytest.mark.parametrize("b,r,d", [(3, 2, 64), (40, 9, 100), (3000, 1, 391)])
+def test_c_abi_preference_strides(lib, b, r, d, more, offset):
+    n, d_pad, up8 = 200, (d + 63) // 64 * 64, (d + 7) // 8 * 8
+    x = torch.zeros(n, d_pad, dtype=torch.float16, device="cuda")
+    x[:, :d] = randn(n, d, dtype=torch.float16, seed=1, scale=0.3)
+    _, q = padded(b, d, d + more, torch.bfloat16, offset, randn(b, d, dtype=torch.bfloat16, seed=2))
+    _, ref = padded(b, d, d + more, torch.float32, offset, randn(b, d, dtype=torch.float32, seed=3))
+    chosen, rej = ids(n, b, seed=4, gone=0.1), ids(n, b, r, seed=5, gone=0.2)
+    _, rejected = padded(b, r, r + 3, torch.int64, 0, rej)
+    loss, weight = torch.full((4,), FILL, device="cuda"), torch.full((4,), FILL, device="cuda")
+    mbuf = torch.full((b * r + 8,), FILL, device="cuda")
+    gbuf = torch.full((b + 1, up8 + 16), FILL, device="cuda")
+    need = size()
+    assert lib.cvs_preference_loss_workspace_size(b, r, ctypes.byref(need)) == 0
+    ws = torch.empty(max(need.value, 256), dtype=torch.uint8, device="cuda")
+    st = lib.cvs_preference_loss(q.data_ptr(), 2, d + more, ref.data_ptr(), 0, d + more, b, d, 1, x.data_ptr(), n, d_pad,
+                                 chosen.data_ptr(), rejected.data_ptr(), r + 3, r, 4.0, 0.1, 1, loss.data_ptr(),
+                                 weight.data_ptr(), mbuf.data_ptr(), gbuf.data_ptr(), up8 + 16, ws.data_ptr(), ws.numel(), stream())
+    assert st == 0, lib.cvs_last_error()
+    want_loss, want_m, want_dq = oracle.preference(q, ref, chosen, rej, x[:, :d], True, 4.0, 0.1, True)
+    unit = lambda v: (v.double() / v.double().norm(dim=1, keepdim=True)).abs()  # noqa: E731
+    xa = x[:, :d].double().abs()
+    sizes = xa[chosen.clamp_min(0)][:, None] + xa[rej.clamp_min(0)]
+    m_err = 4.0 * 150 * E * (sizes * (unit(q) + unit(ref))[:, None]).sum(2)
+    oracle.close(mbuf[: b * r].view(b, r), want_m, m_err + 4 * E * want_m.abs())
+    oracle.close(loss[0], want_loss, m_err.mean() * 2 + 120 * E * want_loss.abs())
+    assert (mbuf[b * r :] == FILL).all() and (loss[1:] == FILL).all() and (weight[1:] == FILL).all() and (gbuf[b] == FILL).all()
+    upstream, dqb = torch.tensor([2.0], device="cuda"), torch.full((b * d + 8,), FILL, device="cuda")
+    assert lib.cvs_preference_grad(gbuf.data_ptr(), up8 + 16, b, d, weight.data_ptr(), upstream.data_ptr(), 0, dqb.data_ptr(), stream()) == 0
+    # Slopes of at most 0.9 x scale, each off by m_err / 4 and 16 e, over sums of r + 2 roundings, twice projected, over |q|.
+    pairs = max(int(((chosen[:, None] >= 0) & (rej >= 0)).sum()), 1)
+    per_row = (4.0 * (0.25 * m_err + 120 * E)[:, :, None] * sizes).sum(1)
+    err = (per_row + unit(q) * (unit(q) * per_row).sum(1, keepdim=True) * 4) / q.double().norm(dim=1, keepdim=True) * 2.0 / pairs
+    oracle.close(dqb[: b * d].view(b, d), 2.0 * want_dq, err)
+    assert (dqb[b * d :] == FILL).all()
+
+
+@pytest.mark.parametrize("rows,cols,more", [(1, 1, 0), (5, 64, 0), (700, 65, 8), (9, 300, 256), (3, 257, 512)])
+def test_c_abi_align_rows(lib, rows, cols, more):
+    _, src = padded(rows, cols, cols + 3, torch.bfloat16, 1, randn(rows, cols, dtype=torch.bfloat16, seed=1))
+    stride = (cols + 7) // 8 * 8 + more
+    buf, dst = padded(rows, cols, stride, torch.bfloat16)
+    assert lib.cvs_align_rows(src.data_ptr(), cols + 3, 2, rows, cols, dst.data_ptr(), stride, stream()) == 0
+    assert torch.equal(dst, src) and (buf[rows * stride :] == FILL).all()
+    behind = buf[: rows * stride].view(rows, stride)[:, cols:]
+    assert ((behind == 0) | (behind == FILL)).all()
