@@ -19,19 +19,20 @@ namespace {
 // Activations
 // ---------------------------------------------------------------------------
 // GELU z Phi(z) = max(z, 0) - |z| Q(|z|) with the tail probability Q(a) = Phi(-a) as
-// 2^P(-a): log2 Q is smooth and nearly quadratic, so a degree-8 polynomial (a
-// least-squares fit on 0 .. 13.3 reweighted towards the smallest largest error, with the
-// error allowed to grow from 6 on) gives Q to 7e-6 relative up to 6, 3e-4 up to 9, 3e-3 up
-// to 11 and 0.12 up to 12.95, where it passes fp32's smallest normal number and becomes
-// zero; bf16, which has fp32's range, sees all of it. For eight multiply-adds and one ex2;
-// the multiply-adds run on pairs (fma.rn.f32x2), two elements an instruction. With erff the
-// epilogue, not the tensor cores, set the pace: 16384 x 768 -> 1536 took 112 us, against
+// 2^P(-a): log2 Q is smooth and nearly quadratic, so a degree-8 polynomial does. It is a
+// least-squares fit on 0 .. 13.3 reweighted towards the smallest largest share of what is
+// allowed: an error of Q that stays a fixed number of roundings of |z| (12 e are reached, e =
+// 2^-24), and 2e-5 of Q itself up to 6, growing to 1e-2 at the end. Reached: 5e-5 of Q up to
+// 6, 5e-4 up to 9, 1.2e-3 up to 11 and 1.4e-2 up to 12.95, where Q passes fp32's smallest
+// normal number and becomes zero; bf16, which has fp32's range, sees all of it. It costs eight
+// multiply-adds, on pairs (fma.rn.f32x2: two elements an instruction), and one ex2. With erff
+// the epilogue, not the tensor cores, set the pace: 16384 x 768 -> 1536 took 112 us, against
 // 47 us without an activation.
 constexpr float kTailEnd = 13.3f;
 constexpr int kTailDegree = 8;
-__device__ constexpr float kTail[kTailDegree + 1] = {-0.9999926686286926f, 1.151314377784729f, -0.4582221210002899f,
-                                                    0.054303329437971115f, 0.008741442114114761f, 0.0010153331095352769f,
-                                                    7.842765626264736e-05f, 3.5550276606954867e-06f, 7.081060005020845e-08f};
+__device__ constexpr float kTail[kTailDegree + 1] = {-0.9999980330467224f, 1.1511892080307007f, -0.4586566388607025f,
+                                                    0.0537852942943573f, 0.00846633780747652f, 0.0009411636856384575f,
+                                                    6.787561142118648e-05f, 2.80283438769402e-06f, 4.9737455043441514e-08f};
 constexpr float kLog2E = 1.4426950408889634f;
 
 // The larger (smaller) of the two; NaN if either is.

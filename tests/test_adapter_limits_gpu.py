@@ -351,6 +351,20 @@ def test_gelu_goes_to_zero(cvs, m):
     oracle.close(dx[:, 0], slope[0], (rel[0] + 2.0**-8) * slope[0].abs() + 1e-37)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("m", [2, 4000])
+def test_gelu_error_is_a_share_of_z(cvs, dtype, m):
+    """Products of two halves are exact pre-activations: over four million of them the GELU is
+    off by its rounding and 16 e of |z| at most (its polynomial 12 e, the exponential's 2 ulp
+    half of 4 e, product and sum e each)."""
+    t = DTYPES[dtype]
+    n = 4_000_000 // m
+    x, w = randn(m, 1, dtype=t, seed=1), randn(n, 1, dtype=t, seed=2, scale=2.0)
+    y = cvs.linear(x, w, activation="gelu")
+    z = x.double() @ w.double().T
+    oracle.close(y, oracle.act(z, "gelu")[0], 16 * E * z.abs())
+
+
 # ---- counts past 32 bits ---------------------------------------------------------------
 def test_counts_past_32_bits_are_refused(cvs):
     """A count of columns or rows is never cut to its low 32 bits."""
